@@ -1,6 +1,7 @@
 """ctypes bindings of the two native libraries (include/agpt_attn.h,
-include/agpt_loss.h and include/agpt_block.h in libagpt_attn.so;
-include/agpt_trie.h in libagpt_trie.so).
+include/agpt_loss.h, include/agpt_block.h, include/agpt_embed.h and
+include/agpt_act8.h in libagpt_attn.so; include/agpt_trie.h in
+libagpt_trie.so).
 
 The attention library is the product path: if it is missing or fails to load,
 every call raises — there is no Python or CPU fallback.
@@ -93,6 +94,36 @@ BLOCK_SYMBOLS = {
     "agpt_norm_bwd": (C.c_int, [_vp] * 10 + [C.c_int64, C.c_int64, C.c_int, _vp]),
     "agpt_norm_workspace_floats": (C.c_int64, [C.c_int]),
     "agpt_relu_bwd": (C.c_int, [_vp] * 5 + [C.c_int64, C.c_int64, C.c_int, _vp]),
+    "agpt_qk_norm_rope_split": (C.c_int, [_vp, C.c_int64] + [_vp] * 6 + [C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int,
+                                                                         C.c_float, C.c_int] + [_vp] * 4),
+    "agpt_qk_norm_rope_split_bwd": (C.c_int, [_vp] * 4 + [C.c_int64] + [_vp] * 6 +
+                                    [C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int, _vp,
+                                     C.c_int64] + [_vp] * 4 + [C.c_int64, _vp]),
+    "agpt_qk_norm_workspace_floats": (C.c_int64, [C.c_int, C.c_int, C.c_int]),
+}
+
+# include/agpt_embed.h (same library as the attention entry points).
+EMBED_SYMBOLS = {
+    "agpt_embed_fwd": (C.c_int, [_vp, _vp, C.c_int, C.c_float, _vp, C.c_int64, C.c_int64, C.c_int, C.c_int, _vp]),
+    "agpt_embed_plan_ints": (C.c_int64, [C.c_int64, C.c_int64]),
+    "agpt_embed_plan_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int64]),
+    "agpt_embed_plan": (C.c_int, [_vp, C.c_int, C.c_int64, C.c_int64, _vp, _vp, C.c_int64, _vp]),
+    "agpt_embed_bwd_workspace_floats": (C.c_int64, [C.c_int64, C.c_int]),
+    "agpt_embed_bwd": (C.c_int, [_vp, C.c_int64, _vp, C.c_float, _vp, _vp, C.c_int64, C.c_int64, C.c_int64, C.c_int,
+                                 C.c_int, _vp]),
+}
+
+# include/agpt_act8.h (same library as the attention entry points).
+ACT8_SYMBOLS = {
+    "agpt_act8_code_bytes": (C.c_int64, [C.c_int64, C.c_int]),
+    "agpt_act8_scale_bytes": (C.c_int64, [C.c_int64, C.c_int]),
+    "agpt_act8_pack": (C.c_int, [_vp, C.c_int64, C.c_int, C.c_int, _vp, _vp, C.c_int64, C.c_int, _vp]),
+    "agpt_act8_unpack": (C.c_int, [_vp, _vp, C.c_int, _vp, C.c_int64, C.c_int, C.c_int64, C.c_int, _vp]),
+    "agpt_act8_wgrad_workspace_floats": (C.c_int64, [C.c_int64, C.c_int, C.c_int]),
+    "agpt_act8_wgrad": (C.c_int, [_vp, C.c_int64, C.c_int, _vp, _vp, C.c_int, _vp, _vp, _vp, C.c_int64, C.c_int64,
+                                  C.c_int, C.c_int, _vp]),
+    "agpt_act8_relu_wgrad": (C.c_int, [_vp, C.c_int64, C.c_int, _vp, _vp, _vp, _vp, C.c_int, _vp, _vp, _vp, C.c_int64,
+                                       C.c_int64, C.c_int, C.c_int, _vp]),
 }
 
 TRIE_SYMBOLS = {
@@ -135,7 +166,8 @@ def _load(name: str, symbols: dict) -> C.CDLL:
 def attn_lib() -> C.CDLL:
     global _attn
     if _attn is None:
-        _attn = _load("libagpt_attn.so", {**ATTN_SYMBOLS, **LOSS_SYMBOLS, **BLOCK_SYMBOLS})
+        _attn = _load("libagpt_attn.so", {**ATTN_SYMBOLS, **LOSS_SYMBOLS, **BLOCK_SYMBOLS,
+                                             **EMBED_SYMBOLS, **ACT8_SYMBOLS})
     return _attn
 
 

@@ -1,6 +1,7 @@
 """Kernels around the trie-attention path in a training step
-(include/agpt_block.h): the projection epilogue (bias + RoPE, in place), the
-row norms and the RMSProp update. Torch CUDA tensors, current stream; no CPU
+(include/agpt_block.h): the projection epilogue (bias + RoPE, in place or with
+the split, with or without a norm of queries and keys), the row norms and the
+RMSProp update. Torch CUDA tensors, current stream; no CPU
 fallback."""
 from __future__ import annotations
 
@@ -16,6 +17,41 @@ def _ptr(t):
 def _stream(t) -> C.c_void_p:
     import torch
     return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+def _launch(device, call) -> None:
+    """Runs a native call with `device` current, and raises on its status."""
+    import torch
+    if device.index == torch.cuda.current_device():
+        _native.check(call())
+    else:
+        with torch.cuda.device(device):
+            _native.check(call())
+
+
+def _check_cuda(name: str, t, device=None) -> None:
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} must be on {device}")
+
+
+def _dtype(name: str, t) -> int:
+    import torch
+    if t.dtype == torch.float32:
+        return _native.AGPT_DTYPE_F32
+    if t.dtype == torch.bfloat16:
+        return _native.AGPT_DTYPE_BF16
+    raise ValueError(f"{name} must be float32 or bfloat16")
+
+
+def _rows(name: str, t) -> int:
+    """The row stride, in elements, of a 2-D tensor whose rows are contiguous."""
+    if t.dim() == 2 and t.numel() == 0:
+        return max(1, t.shape[1])
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise ValueError(f"{name} must be 2-D with contiguous rows that do not overlap")
+    return t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1])
 
 
 def bias_rope_(x, bias=None, positions=None, cos_t=None, sin_t=None, n_heads: int = 1):
@@ -48,6 +84,80 @@ def bias_rope_split(qkv, bias=None, positions=None, cos_t=None, sin_t=None, n_he
         _ptr(qkv), _ptr(bias), _ptr(positions), _ptr(cos_t), _ptr(sin_t), seq, T, n_heads, D // n_heads,
         _ptr(q), _ptr(k), _ptr(v), _stream(qkv)))
     return q, k, v
+
+
+def _qk_args(qkv, wq, wk, bias, positions, cos_t, sin_t, n_heads, n_kv_heads):
+    """Checks what the norm's two directions share; the row's head counts and sizes."""
+    import torch
+    _check_cuda("qkv", qkv)
+    dt, ld = _dtype("qkv", qkv), _rows("qkv", qkv)
+    Hk = n_heads if n_kv_heads is None else n_kv_heads
+    if n_heads < 1 or Hk < 1:
+        raise ValueError("n_heads and n_kv_heads must be at least 1")
+    T, width = qkv.shape
+    if width < 1 or width % (n_heads + 2 * Hk):
+        raise ValueError("qkv's width must be a multiple of n_heads + 2 n_kv_heads")
+    hd = width // (n_heads + 2 * Hk)
+    seq = 0
+    small = [("wq", wq, hd), ("wk", wk, hd)] + ([("bias", bias, width)] if bias is not None else [])
+    if cos_t is not None:
+        if sin_t is None or positions is None:
+            raise ValueError("the rotation needs cos_t, sin_t and positions")
+        seq = cos_t.shape[0]
+        small += [("cos_t", cos_t, seq * hd), ("sin_t", sin_t, seq * hd)]
+        _check_cuda("positions", positions, qkv.device)
+        if positions.dtype != torch.int32 or positions.shape != (T,) or not positions.is_contiguous():
+            raise ValueError("positions must be a contiguous int32 [T] tensor")
+    for name, t, n in small:
+        _check_cuda(name, t, qkv.device)
+        if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous float32 with {n} elements")
+    return dt, ld, T, hd, Hk, seq
+
+
+def qk_norm_rope_split(qkv, wq, wk, bias=None, positions=None, cos_t=None, sin_t=None, n_heads: int = 1,
+                       n_kv_heads: int | None = None, eps: float = 1e-5):
+    """bias_rope_split with an RMSNorm of every query and key head in front of
+    the rotation: qkv [T, (n_heads + 2 n_kv_heads) hd] (fp32 or bf16, rows may
+    be strided) -> contiguous q [T, n_heads hd], k and v [T, n_kv_heads hd].
+    wq, wk [hd] and bias are fp32; n_kv_heads None: as many as n_heads."""
+    import torch
+    dt, ld, T, hd, Hk, seq = _qk_args(qkv, wq, wk, bias, positions, cos_t, sin_t, n_heads, n_kv_heads)
+    q, k, v = (torch.empty(T, h * hd, device=qkv.device, dtype=qkv.dtype) for h in (n_heads, Hk, Hk))
+    _launch(qkv.device, lambda: _native.attn_lib().agpt_qk_norm_rope_split(
+        _ptr(qkv), ld, _ptr(bias), _ptr(wq), _ptr(wk), _ptr(positions), _ptr(cos_t), _ptr(sin_t), seq, T, n_heads, Hk, hd,
+        C.c_float(eps), dt, _ptr(q), _ptr(k), _ptr(v), _stream(qkv)))
+    return q, k, v
+
+
+def qk_norm_rope_split_bwd(dq, dk, dv, qkv, wq, wk, bias=None, positions=None, cos_t=None, sin_t=None,
+                           n_heads: int = 1, n_kv_heads: int | None = None, eps: float = 1e-5, out=None):
+    """(dqkv, dwq, dwk, dbias or None) of qk_norm_rope_split from the gradients
+    of its outputs; weights' and bias' gradients are fp32 sums in a fixed order.
+    cos_t None: dq and dk are gradients in front of the rotation already (as
+    TrieAttention.backward returns them when it is given the tables)."""
+    import torch
+    dt, ld, T, hd, Hk, seq = _qk_args(qkv, wq, wk, bias, positions, cos_t, sin_t, n_heads, n_kv_heads)
+    for name, t, h in (("dq", dq, n_heads), ("dk", dk, Hk), ("dv", dv, Hk)):
+        _check_cuda(name, t, qkv.device)
+        if t.shape != (T, h * hd) or t.dtype != qkv.dtype or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous [T, {h * hd}] tensor of qkv's type")
+    if out is None:
+        out = torch.empty(T, qkv.shape[1], device=qkv.device, dtype=qkv.dtype)
+    _check_cuda("out", out, qkv.device)
+    if out.shape != qkv.shape or out.dtype != qkv.dtype:
+        raise ValueError("out must be shaped as qkv and of its type")
+    ld_out = _rows("out", out)
+    lib = _native.attn_lib()
+    n = lib.agpt_qk_norm_workspace_floats(n_heads, Hk, hd)
+    ws = torch.empty(n, device=qkv.device, dtype=torch.float32)
+    dwq, dwk = (torch.empty(hd, device=qkv.device, dtype=torch.float32) for _ in range(2))
+    db = torch.empty(qkv.shape[1], device=qkv.device, dtype=torch.float32) if bias is not None else None
+    _launch(qkv.device, lambda: lib.agpt_qk_norm_rope_split_bwd(
+        _ptr(dq), _ptr(dk), _ptr(dv), _ptr(qkv), ld, _ptr(bias), _ptr(wq), _ptr(wk), _ptr(positions), _ptr(cos_t),
+        _ptr(sin_t), seq, T, n_heads, Hk, hd, C.c_float(eps), dt, _ptr(out), ld_out, _ptr(dwq), _ptr(dwk), _ptr(db),
+        _ptr(ws), n, _stream(qkv)))
+    return out, dwq, dwk, db
 
 
 def rmsprop_(params, grads, sq_avg, lr: float, beta: float, eps: float = 1e-8):

@@ -42,7 +42,8 @@ HIP_FLAGS = [
     "-Wno-unused-result",
 ]
 
-HIP_SOURCES = ["trie_attn.hip", "varlen_attn.hip", "agpt_loss.hip", "agpt_block.hip"]
+HIP_SOURCES = ["trie_attn.hip", "varlen_attn.hip", "agpt_loss.hip", "agpt_block.hip", "agpt_embed.hip",
+               "agpt_qknorm.hip", "agpt_act8.hip"]
 
 # Per-source flags. The trie kernels are scheduled for instruction-level
 # parallelism: the block pair's S/dP products, softmax and dV/dK/dQ products

@@ -1,0 +1,570 @@
+// agpt_act8.hip — 8-bit activation checkpoints (gfx950): packing, unpacking,
+// and the weight gradient of a linear layer from its checkpointed input.
+//
+// Packing and unpacking are HBM-bound: a lane holds four columns of eight rows
+// (eight 16-byte loads in flight), eight lanes share a block of 32 columns and
+// its scale, and a lane's codes are 32 consecutive bytes.
+//
+// The weight gradient dW[o][i] = sum_t dy[t][o] val[t][i] contracts over rows
+// that are far apart in memory. A matrix instruction takes from each lane
+// eight consecutive steps of the contraction for one row of its operand, so a
+// lane simply loads eight rows of its own columns: no transposition, no LDS,
+// and any assignment of columns to operand rows is as good as another, so
+// lane l takes columns 2l, 2l+1 of dy and 4l..4l+3 of the checkpoint, whose
+// bytes lie together in its layout. A wave owns a 64 x 128 tile of dW (eight
+// 32x32 accumulators) over a chunk of rows and needs no other wave.
+//   val has at most 8 significant bits: exact in bf16.
+//   an fp32 dy is cut into three bf16 parts by truncation, 8 + 8 + 8 bits,
+//   which add up to it exactly: three products at the bf16 rate instead of one
+//   at the fp32 rate, 1/16 of it.
+// Chunks leave partial tiles, folded in chunk order.
+
+#include "rows.h"
+#include "../../include/agpt_act8.h"
+
+#include <type_traits>
+
+namespace {
+
+using namespace agpt_rows;
+
+constexpr int kThreads = 256;
+constexpr int kBlock = 32;  // columns under one scale
+constexpr int kRows = 8;    // rows of a layout block
+
+int64_t row_blocks(int64_t T) { return (T + kRows - 1) / kRows; }
+
+// ---- pack -------------------------------------------------------------------
+// The scale byte of a block whose largest magnitude has the bits `m`: with
+// top = 127 = 1.984375 * 2^6 (255 = 1.9921875 * 2^7), the exponent of m less
+// that of top, one more if m's mantissa is above top's. 255 for infinity, NaN and
+// what would need s above 2^120, whose codes' values need not be finite.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t m, bool relu) {
+  if (m >= 0x7f800000u) return 255u;
+  const int e = static_cast<int>((m + (relu ? 0x0000ffffu : 0x0001ffffu)) >> 23) - (relu ? 7 : 6);
+  return e > 247 ? 255u : static_cast<uint32_t>(e < 1 ? 1 : e);
+}
+
+template <int kCtrl>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+  const uint32_t o = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, 0xf, 0xf, false));
+  return v > o ? v : o;
+}
+
+// Magnitude bits that count for the block's scale: |x|, or x where it is above
+// zero (what is not finite always counts).
+__device__ __forceinline__ uint32_t magnitude(float x, bool relu) {
+  const uint32_t b = __float_as_uint(x), m = b & 0x7fffffffu;
+  return relu && (b >> 31) && m < 0x7f800000u ? 0u : m;
+}
+
+__device__ __forceinline__ uint32_t code_of(float x, float inv, bool nan_block, bool relu) {
+  const uint32_t b = __float_as_uint(x);
+  const bool above = !(b >> 31) && b != 0u && b <= 0x7f800000u;
+  if (nan_block) return relu ? static_cast<uint32_t>(above) : 128u;
+  const float r = rintf(x * inv);
+  if (!relu) return static_cast<uint32_t>(static_cast<int>(r) + 128);
+  const uint32_t c = static_cast<uint32_t>(static_cast<int>(r));
+  return above ? (c < 1u ? 1u : c) : 0u;
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads) void pack_kernel(const T* __restrict__ x, int64_t ld, uint8_t* __restrict__ codes,
+                                                        uint8_t* __restrict__ scales, int64_t rows, int quads,
+                                                        int64_t items, int gx, bool relu) {
+  for (int64_t i = static_cast<int64_t>(block_x()) * kThreads + thread_x(); i < items;
+       i += static_cast<int64_t>(gx) * kThreads) {
+    const int64_t rb = i / quads;
+    const int q = static_cast<int>(i - rb * quads);
+    const T* p = x + rb * kRows * ld + 4 * q;
+    const int live = rows - rb * kRows < kRows ? static_cast<int>(rows - rb * kRows) : kRows;
+    float v[kRows][4];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[r][j] = 0.0f;
+      if (r < live) {
+        if constexpr (V == 4) {
+          load_row<4>(p + r * ld, v[r]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[r][j] = agpt::to_f32(p[r * ld + j]);
+        }
+      }
+    }
+    uint32_t c[kRows], sb[2] = {0u, 0u};
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t a = magnitude(v[r][j], relu);
+        m = m > a ? m : a;
+      }
+      m = dpp_max<0x141>(dpp_max<0x1B>(dpp_max<0xB1>(m)));  // over the block's eight lanes
+      const uint32_t e = scale_byte(m, relu);
+      const float inv = __uint_as_float((e == 255u ? 0u : 254u - e) << 23);  // 1 / s = 2^(127 - e)
+      uint32_t w = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w |= code_of(v[r][j], inv, e == 255u, relu) << (8 * j);
+      c[r] = w;
+      sb[r / 4] |= e << (8 * (r % 4));
+    }
+    uint4* out = reinterpret_cast<uint4*>(codes + i * (4 * kRows));
+    out[0] = uint4{c[0], c[1], c[2], c[3]};
+    out[1] = uint4{c[4], c[5], c[6], c[7]};
+    if (q % 8 == 0) *reinterpret_cast<uint2*>(scales + (i / 8) * kRows) = uint2{sb[0], sb[1]};
+  }
+}
+
+// ---- values -------------------------------------------------------------------
+// s = 2^(e - 127); e = 255 reads as infinity, and every value as NaN: code * inf - zero * inf.
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+template <int kByte>
+__device__ __forceinline__ float byte_f(uint32_t w) {
+  return static_cast<float>((w >> (8 * kByte)) & 0xffu);
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads) void unpack_kernel(const uint8_t* __restrict__ codes,
+                                                          const uint8_t* __restrict__ scales, T* __restrict__ x,
+                                                          int64_t ld, int64_t rows, int quads, int64_t items, int gx,
+                                                          float zero) {
+  for (int64_t i = static_cast<int64_t>(block_x()) * kThreads + thread_x(); i < items;
+       i += static_cast<int64_t>(gx) * kThreads) {
+    const int64_t rb = i / quads;
+    const int q = static_cast<int>(i - rb * quads);
+    const uint4 a = reinterpret_cast<const uint4*>(codes + i * (4 * kRows))[0];
+    const uint4 b = reinterpret_cast<const uint4*>(codes + i * (4 * kRows))[1];
+    const uint2 sc = *reinterpret_cast<const uint2*>(scales + (rb * (quads / 8) + q / 8) * kRows);
+    const uint32_t c[kRows] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    const int live = rows - rb * kRows < kRows ? static_cast<int>(rows - rb * kRows) : kRows;
+    T* p = x + rb * kRows * ld + 4 * q;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const float s = scale_of(((r < 4 ? sc.x : sc.y) >> (8 * (r % 4))) & 0xffu), z = -zero * s;
+      const float v[4] = {fmaf(byte_f<0>(c[r]), s, z), fmaf(byte_f<1>(c[r]), s, z), fmaf(byte_f<2>(c[r]), s, z),
+                          fmaf(byte_f<3>(c[r]), s, z)};
+      if (r < live) {
+        if constexpr (V == 4) {
+          store_row<4>(p + r * ld, v);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float one[1] = {v[j]};
+            store_row<1>(p + r * ld + j, one);
+          }
+        }
+      }
+    }
+  }
+}
+
+// ---- weight gradient --------------------------------------------------------------
+constexpr int kTileO = 64, kTileI = 128, kStep = 16;  // a wave's tile of dW, rows of a step
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// The upper halves of two words as a pair of bf16, the first one low.
+__device__ __forceinline__ uint32_t high_pair(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+__device__ __forceinline__ uint32_t low_pair(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+
+struct Grad {
+  int64_t rows, ld, chunk_rows;
+  int out, in, tiles_o, tiles_i, chunks;
+  float zero;
+};
+
+// What a lane holds of a step: its eight rows of two columns of dy, of four
+// code columns with their scales, and of the ReLU's codes.
+template <typename T>
+struct Raw {
+  uint32_t a[kRows][sizeof(T) == 4 ? 2 : 1];
+  uint4 c0, c1;
+  uint2 sc;
+  uint4 h0, h1;
+};
+
+// kPair: columns 2l and 2l + 1 in one load (dy aligned to the pair, an even
+// width); otherwise columns l and l + 32.
+template <typename T, bool kPair, bool kRelu>
+__global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(const T* __restrict__ dy, const uint8_t* __restrict__ hc,
+                                                            T* __restrict__ dh, const uint8_t* __restrict__ codes,
+                                                            const uint8_t* __restrict__ scales,
+                                                            float* __restrict__ dw, float* __restrict__ db,
+                                                            int64_t db_ld, Grad g) {
+  const int lane = thread_x() & 63, l = lane & 31, half = lane >> 5;
+  const int64_t unit = static_cast<int64_t>(block_x()) * (kThreads / 64) + (thread_x() >> 6);
+  const int tiles = g.tiles_o * g.tiles_i;
+  const int chunk = static_cast<int>(unit / tiles), tile = static_cast<int>(unit - static_cast<int64_t>(chunk) * tiles);
+  if (chunk >= g.chunks) return;
+  const int to = tile / g.tiles_i, ti = tile - to * g.tiles_i;
+  const int o0 = to * kTileO, i0 = ti * kTileI;
+  const int64_t t0 = chunk * g.chunk_rows, t1 = t0 + g.chunk_rows < g.rows ? t0 + g.chunk_rows : g.rows;
+  const int oa = kPair ? o0 + 2 * l : o0 + l, ob = kPair ? oa + 1 : oa + 32;  // the lane's columns of dy
+  const bool ina = oa < g.out, inb = ob < g.out;
+  const int quads = g.in / 4, quad = i0 / 4 + l;
+  const bool inq = quad < quads;
+  const int64_t blocks = (g.rows + kRows - 1) / kRows;
+
+  f32x16 acc[2][4];
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[p][j][r] = 0.0f;
+  float sum_a = 0.0f, sum_b = 0.0f;
+  const bool sums = db != nullptr && ti == 0, writes = kRelu && ti == 0;
+
+  auto load = [&](int64_t t, Raw<T>& w) {
+    const int64_t first = t + half * kRows;
+    const int64_t rb = first / kRows;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const bool row = first + r < t1;
+      const T* p = dy + (first + r) * g.ld;
+      if constexpr (sizeof(T) == 4) {
+        w.a[r][0] = w.a[r][1] = 0u;
+        if constexpr (kPair) {
+          if (row && ina) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p + oa);
+            w.a[r][0] = v.x;
+            w.a[r][1] = v.y;
+          }
+        } else {
+          if (row && ina) w.a[r][0] = __float_as_uint(p[oa]);
+          if (row && inb) w.a[r][1] = __float_as_uint(p[ob]);
+        }
+      } else {
+        w.a[r][0] = 0u;
+        if constexpr (kPair) {
+          if (row && ina) w.a[r][0] = *reinterpret_cast<const uint32_t*>(p + oa);
+        } else {
+          if (row && ina) w.a[r][0] = p[oa].bits;
+          if (row && inb) w.a[r][0] |= static_cast<uint32_t>(p[ob].bits) << 16;
+        }
+      }
+    }
+    // no block of the checkpoint, or no such columns: scale 0, value 0
+    const bool live = inq && rb < blocks;
+    w.c0 = w.c1 = uint4{0u, 0u, 0u, 0u};
+    w.sc = uint2{0u, 0u};
+    if (live) {
+      const uint4* c = reinterpret_cast<const uint4*>(codes + (rb * quads + quad) * (4 * kRows));
+      w.c0 = c[0];
+      w.c1 = c[1];
+      w.sc = *reinterpret_cast<const uint2*>(scales + (rb * (quads / 8) + quad / 8) * kRows);
+    }
+    if constexpr (kRelu) {
+      w.h0 = w.h1 = uint4{0u, 0u, 0u, 0u};
+      if (ina && rb < blocks) {
+        const uint4* c = reinterpret_cast<const uint4*>(hc + (rb * (g.out / 4) + oa / 4) * (4 * kRows));
+        w.h0 = c[0];
+        w.h1 = c[1];
+      }
+    }
+  };
+
+  auto step = [&](int64_t t, Raw<T>& w) {
+    if constexpr (kRelu) {
+      const uint32_t h[kRows] = {w.h0.x, w.h0.y, w.h0.z, w.h0.w, w.h1.x, w.h1.y, w.h1.z, w.h1.w};
+      const int sh = (l & 1) * 16;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const uint32_t m = h[r] >> sh;
+        if constexpr (sizeof(T) == 4) {
+          w.a[r][0] = (m & 0xffu) ? w.a[r][0] : 0u;
+          w.a[r][1] = (m & 0xff00u) ? w.a[r][1] : 0u;
+        } else {
+          w.a[r][0] &= ((m & 0xffu) ? 0xffffu : 0u) | ((m & 0xff00u) ? 0xffff0000u : 0u);
+        }
+        if (writes && ina && t + half * kRows + r < t1) {
+          T* p = dh + (t + half * kRows + r) * g.out + oa;
+          if constexpr (sizeof(T) == 4) *reinterpret_cast<uint2*>(p) = uint2{w.a[r][0], w.a[r][1]};
+          else *reinterpret_cast<uint32_t*>(p) = w.a[r][0];
+        }
+      }
+    }
+    if (sums) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        if constexpr (sizeof(T) == 4) {
+          sum_a += __uint_as_float(w.a[r][0]);
+          sum_b += __uint_as_float(w.a[r][1]);
+        } else {
+          sum_a += __uint_as_float(w.a[r][0] << 16);
+          sum_b += __uint_as_float(w.a[r][0] & 0xffff0000u);
+        }
+      }
+    }
+    // the four code columns as bf16, eight rows each
+    uint4 b[4];
+    {
+      const uint32_t c[kRows] = {w.c0.x, w.c0.y, w.c0.z, w.c0.w, w.c1.x, w.c1.y, w.c1.z, w.c1.w};
+      uint32_t v[4][kRows / 2];
+#pragma unroll
+      for (int r = 0; r < kRows; r += 2) {
+        const uint32_t sw = r < 4 ? w.sc.x : w.sc.y;
+        const float s0 = scale_of((sw >> (8 * (r % 4))) & 0xffu), z0 = -g.zero * s0;
+        const float s1 = scale_of((sw >> (8 * (r % 4 + 1))) & 0xffu), z1 = -g.zero * s1;
+        auto pair = [&](float x, float y) {
+          return high_pair(__float_as_uint(fmaf(x, s0, z0)), __float_as_uint(fmaf(y, s1, z1)));
+        };
+        v[0][r / 2] = pair(byte_f<0>(c[r]), byte_f<0>(c[r + 1]));
+        v[1][r / 2] = pair(byte_f<1>(c[r]), byte_f<1>(c[r + 1]));
+        v[2][r / 2] = pair(byte_f<2>(c[r]), byte_f<2>(c[r + 1]));
+        v[3][r / 2] = pair(byte_f<3>(c[r]), byte_f<3>(c[r + 1]));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = uint4{v[j][0], v[j][1], v[j][2], v[j][3]};
+    }
+    auto products = [&](int p, uint4 a) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        acc[p][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b[j]),
+                                                            acc[p][j], 0, 0, 0);
+    };
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      uint32_t m[kRows / 2];
+      if constexpr (sizeof(T) == 4) {
+        // three parts by truncation; each remainder is exact
+        float x[kRows];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) x[r] = __uint_as_float(w.a[r][p]);
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+#pragma unroll
+          for (int r = 0; r < kRows; r += 2) m[r / 2] = high_pair(__float_as_uint(x[r]), __float_as_uint(x[r + 1]));
+          if (part < 2) {
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) x[r] -= __uint_as_float(__float_as_uint(x[r]) & 0xffff0000u);
+          }
+          products(p, uint4{m[0], m[1], m[2], m[3]});
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < kRows; r += 2)
+          m[r / 2] = p ? high_pair(w.a[r][0], w.a[r + 1][0]) : low_pair(w.a[r][0], w.a[r + 1][0]);
+        products(p, uint4{m[0], m[1], m[2], m[3]});
+      }
+    }
+  };
+
+  Raw<T> w0, w1;
+  load(t0, w0);
+  for (int64_t t = t0; t < t1; t += 2 * kStep) {
+    if (t + kStep < t1) load(t + kStep, w1);
+    step(t, w0);
+    if (t + kStep < t1) {
+      if (t + 2 * kStep < t1) load(t + 2 * kStep, w0);
+      step(t + kStep, w1);
+    }
+  }
+
+  // accumulator register r of lane (l, half): operand row 8 (r / 4) + 4 half + r % 4 of dy, column l of the codes
+  float* out = dw + static_cast<int64_t>(chunk) * g.out * g.in;
+  if (inq) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int m = 8 * (r / 4) + 4 * half + r % 4;
+        const int o = kPair ? o0 + 2 * m + p : o0 + m + 32 * p;
+        if (o < g.out)
+          *reinterpret_cast<float4*>(out + static_cast<int64_t>(o) * g.in + 4 * quad) =
+              float4{acc[p][0][r], acc[p][1][r], acc[p][2][r], acc[p][3][r]};
+      }
+  }
+  if (sums) {
+    sum_a += __shfl_xor(sum_a, 32);
+    sum_b += __shfl_xor(sum_b, 32);
+    if (half == 0) {
+      if (ina) db[chunk * db_ld + oa] = sum_a;
+      if (inb) db[chunk * db_ld + ob] = sum_b;
+    }
+  }
+}
+
+__global__ __launch_bounds__(kFoldThreads) void wgrad_fold_kernel(const float* __restrict__ part, int64_t n,
+                                                                  const float* __restrict__ part_b, int64_t ldb,
+                                                                  int chunks, int out, float* __restrict__ dw,
+                                                                  float* __restrict__ db, int wblocks) {
+  const int blk = block_x();
+  if (blk < wblocks) {
+    fold_columns(part + static_cast<int64_t>(blk) * 64, n, chunks,
+                 n - static_cast<int64_t>(blk) * 64 < 64 ? static_cast<int>(n - static_cast<int64_t>(blk) * 64) : 64, 0,
+                 dw + static_cast<int64_t>(blk) * 64);
+  } else {
+    fold_columns(part_b, ldb, chunks, out, blk - wblocks, db);
+  }
+}
+
+constexpr int kUnits = 2048;      // waves: two per SIMD
+constexpr int kMinRows = 64;      // of a chunk
+constexpr int kMaxWidth = 32768;
+
+struct Plan {
+  int tiles_o, tiles_i, chunks;
+  int64_t chunk_rows, db_ld;
+};
+Plan plan_of(int64_t T, int out, int in) {
+  Plan p;
+  p.tiles_o = (out + kTileO - 1) / kTileO;
+  p.tiles_i = (in + kTileI - 1) / kTileI;
+  const int64_t tiles = static_cast<int64_t>(p.tiles_o) * p.tiles_i;
+  int64_t chunks = kUnits / tiles;
+  if (chunks > (T + kMinRows - 1) / kMinRows) chunks = (T + kMinRows - 1) / kMinRows;
+  if (chunks < 1) chunks = 1;
+  p.chunk_rows = ((T + chunks - 1) / chunks + kStep - 1) / kStep * kStep;
+  if (p.chunk_rows < kStep) p.chunk_rows = kStep;
+  p.chunks = static_cast<int>((T + p.chunk_rows - 1) / p.chunk_rows);
+  if (p.chunks < 1) p.chunks = 1;
+  p.db_ld = (out + 3) / 4 * 4;
+  return p;
+}
+
+int check(const char* what, int64_t T, int64_t ld, int width, int W, int dtype) {
+  if (T < 0 || width < 1) return invalid(what, "T < 0 or a width below 1");
+  if (W < kBlock || W % kBlock != 0) return invalid(what, "a checkpoint's width must be a multiple of 32");
+  if (W > kMaxWidth || width > kMaxWidth) {
+    return agpt_internal_set_error(AGPT_ERR_UNSUPPORTED, "agpt_act8: widths above 32768 are not supported");
+  }
+  if (ld < width) return invalid(what, "row stride smaller than a row");
+  if (dtype != AGPT_DTYPE_F32 && dtype != AGPT_DTYPE_BF16) return invalid(what, "unknown dtype");
+  return AGPT_OK;
+}
+
+int grid_of(int64_t items) {
+  const int64_t need = (items + kThreads - 1) / kThreads;
+  return static_cast<int>(need < 4096 ? need : 4096);
+}
+
+int wgrad(const char* what, const void* dy, int64_t ld, int dtype, const uint8_t* hc, void* dh, const uint8_t* codes,
+          const uint8_t* scales, int relu, float* dw, float* db, float* ws, int64_t ws_floats, int64_t T, int out, int in,
+          void* stream) {
+  if (const int rc = check(what, T, ld, out, in, dtype)) return rc;
+  if (!dw || !ws || (T > 0 && (!dy || !codes || !scales))) return invalid(what, "null pointer");
+  if (ws_floats < agpt_act8_wgrad_workspace_floats(T, out, in))
+    return invalid(what, "workspace smaller than agpt_act8_wgrad_workspace_floats");
+  const int es = dtype == AGPT_DTYPE_F32 ? 4 : 2;
+  if (!aligned(codes, 16) || !aligned(scales, 16) || !aligned(dw, 16) || !aligned(db, 16) || !aligned(ws, 16))
+    return invalid(what, "codes, scales, dw, db and workspace must be 16-byte aligned");
+  if (!aligned(dy, es)) return invalid(what, "dy is not aligned to its elements");
+  const bool pair = out % 2 == 0 && ld % 2 == 0 && aligned(dy, 2 * es);
+  const Plan p = plan_of(T, out, in);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t n = static_cast<int64_t>(out) * in;
+  const bool direct = p.chunks == 1;
+  float* part = direct ? dw : ws;
+  float* part_b = !db ? nullptr : (direct ? db : ws + static_cast<int64_t>(p.chunks) * n);
+  const Grad g{T, ld, p.chunk_rows, out, in, p.tiles_o, p.tiles_i, p.chunks, relu ? 0.0f : 128.0f};
+  const int64_t units = static_cast<int64_t>(p.chunks) * p.tiles_o * p.tiles_i;
+  const dim3 grid(static_cast<unsigned>((units + kThreads / 64 - 1) / (kThreads / 64)));
+  auto go = [&](auto e, auto pc, auto rc) {
+    using E = decltype(e);
+    hipLaunchKernelGGL((wgrad_kernel<E, decltype(pc)::value, decltype(rc)::value>), grid, dim3(kThreads), 0, st,
+                       static_cast<const E*>(dy), hc, static_cast<E*>(dh), codes, scales, part, part_b, p.db_ld, g);
+  };
+  auto kinds = [&](auto e) {
+    if (hc) go(e, std::true_type{}, std::true_type{});
+    else if (pair) go(e, std::true_type{}, std::false_type{});
+    else go(e, std::false_type{}, std::false_type{});
+  };
+  if (dtype == AGPT_DTYPE_F32) kinds(float{});
+  else kinds(bf16_t{});
+  if (const int rc = launch_status(what)) return rc;
+  if (direct) return AGPT_OK;
+  const int wblocks = static_cast<int>((n + 63) / 64), bblocks = db ? (out + 63) / 64 : 0;
+  hipLaunchKernelGGL(wgrad_fold_kernel, dim3(wblocks + bblocks), dim3(kFoldThreads), 0, st, part, n, part_b, p.db_ld,
+                     p.chunks, out, dw, db, wblocks);
+  return launch_status(what);
+}
+
+}  // namespace
+
+extern "C" int64_t agpt_act8_code_bytes(int64_t T, int W) { return T < 0 || W < 1 ? 0 : row_blocks(T) * kRows * W; }
+extern "C" int64_t agpt_act8_scale_bytes(int64_t T, int W) {
+  return T < 0 || W < 1 ? 0 : row_blocks(T) * kRows * (W / kBlock);
+}
+
+extern "C" int agpt_act8_pack(const void* x, int64_t ld_x, int dtype, int relu, uint8_t* codes, uint8_t* scales, int64_t T,
+                              int W, void* stream) {
+  const char* what = "agpt_act8_pack";
+  if (const int rc = check(what, T, ld_x, W, W, dtype)) return rc;
+  if (T == 0) return AGPT_OK;
+  if (!x || !codes || !scales) return invalid(what, "null pointer");
+  const int es = dtype == AGPT_DTYPE_F32 ? 4 : 2;
+  if (!aligned(codes, 16) || !aligned(scales, 16)) return invalid(what, "codes and scales must be 16-byte aligned");
+  if (!aligned(x, es)) return invalid(what, "x is not aligned to its elements");
+  const int quads = W / 4;
+  const int64_t items = row_blocks(T) * quads;
+  const int gx = grid_of(items);
+  const bool wide = ld_x % 4 == 0 && aligned(x, 4 * es);
+  auto go = [&](auto e, auto vc) {
+    using E = decltype(e);
+    hipLaunchKernelGGL((pack_kernel<E, decltype(vc)::value>), dim3(gx), dim3(kThreads), 0, static_cast<hipStream_t>(stream),
+                       static_cast<const E*>(x), ld_x, codes, scales, T, quads, items, gx, relu != 0);
+  };
+  using W4 = std::integral_constant<int, 4>;
+  using W1 = std::integral_constant<int, 1>;
+  if (dtype == AGPT_DTYPE_F32) wide ? go(float{}, W4{}) : go(float{}, W1{});
+  else wide ? go(bf16_t{}, W4{}) : go(bf16_t{}, W1{});
+  return launch_status(what);
+}
+
+extern "C" int agpt_act8_unpack(const uint8_t* codes, const uint8_t* scales, int relu, void* x, int64_t ld_x, int dtype,
+                                int64_t T, int W, void* stream) {
+  const char* what = "agpt_act8_unpack";
+  if (const int rc = check(what, T, ld_x, W, W, dtype)) return rc;
+  if (T == 0) return AGPT_OK;
+  if (!x || !codes || !scales) return invalid(what, "null pointer");
+  const int es = dtype == AGPT_DTYPE_F32 ? 4 : 2;
+  if (!aligned(codes, 16) || !aligned(scales, 16)) return invalid(what, "codes and scales must be 16-byte aligned");
+  if (!aligned(x, es)) return invalid(what, "x is not aligned to its elements");
+  const int quads = W / 4;
+  const int64_t items = row_blocks(T) * quads;
+  const int gx = grid_of(items);
+  const bool wide = ld_x % 4 == 0 && aligned(x, 4 * es);
+  auto go = [&](auto e, auto vc) {
+    using E = decltype(e);
+    hipLaunchKernelGGL((unpack_kernel<E, decltype(vc)::value>), dim3(gx), dim3(kThreads), 0, static_cast<hipStream_t>(stream),
+                       codes, scales, static_cast<E*>(x), ld_x, T, quads, items, gx, relu ? 0.0f : 128.0f);
+  };
+  using W4 = std::integral_constant<int, 4>;
+  using W1 = std::integral_constant<int, 1>;
+  if (dtype == AGPT_DTYPE_F32) wide ? go(float{}, W4{}) : go(float{}, W1{});
+  else wide ? go(bf16_t{}, W4{}) : go(bf16_t{}, W1{});
+  return launch_status(what);
+}
+
+// One partial dW and db per chunk.
+extern "C" int64_t agpt_act8_wgrad_workspace_floats(int64_t T, int out_width, int in_width) {
+  if (T < 0 || out_width < 1 || in_width < 1) return 0;
+  const Plan p = plan_of(T, out_width, in_width);
+  return p.chunks * (static_cast<int64_t>(out_width) * in_width + p.db_ld);
+}
+
+extern "C" int agpt_act8_wgrad(const void* dy, int64_t ld_dy, int dtype, const uint8_t* codes, const uint8_t* scales,
+                               int relu, float* dw, float* db, float* workspace, int64_t workspace_floats, int64_t T,
+                               int out_width, int in_width, void* stream) {
+  return wgrad("agpt_act8_wgrad", dy, ld_dy, dtype, nullptr, nullptr, codes, scales, relu, dw, db, workspace,
+               workspace_floats, T, out_width, in_width, stream);
+}
+
+extern "C" int agpt_act8_relu_wgrad(const void* dh_in, int64_t ld_dh_in, int dtype, const uint8_t* h_codes, void* dh,
+                                    const uint8_t* codes, const uint8_t* scales, int relu, float* dw, float* db,
+                                    float* workspace, int64_t workspace_floats, int64_t T, int out_width, int in_width,
+                                    void* stream) {
+  const char* what = "agpt_act8_relu_wgrad";
+  if (const int rc = check(what, T, ld_dh_in, out_width, out_width, dtype)) return rc;
+  if (T > 0 && (!h_codes || !dh || !dh_in)) return invalid(what, "null pointer");
+  const int es = dtype == AGPT_DTYPE_F32 ? 4 : 2;
+  if (!aligned(dh_in, 16) || !aligned(dh, 16) || !aligned(h_codes, 16) || ld_dh_in * es % 16 != 0)
+    return invalid(what, "dh_in, dh and h_codes must be 16-byte aligned, rows of dh_in too");
+  if (T > 0 && dh == dh_in) return invalid(what, "dh must not overlap dh_in");
+  return wgrad(what, dh_in, ld_dh_in, dtype, T > 0 ? h_codes : nullptr, dh, codes, scales, relu, dw, db, workspace,
+               workspace_floats, T, out_width, in_width, stream);
+}

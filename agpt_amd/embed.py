@@ -1,0 +1,92 @@
+"""Token embedding with scaling, and its gradient by sorted tokens
+(include/agpt_embed.h). Torch CUDA tensors, current stream; no CPU fallback.
+
+Tokens are int32 or int64; a token outside [0, vocab) is padding: its row of x
+is zero and its row of dx counts nowhere. Sums run in a fixed order: two calls
+give the same bytes.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _native
+from .block import _check_cuda, _dtype, _launch, _ptr, _rows, _stream
+
+_BITS = {torch.int32: 32, torch.int64: 64}
+
+
+def _tokens(tokens) -> int:
+    _check_cuda("tokens", tokens)
+    if tokens.dtype not in _BITS or tokens.dim() != 1 or not tokens.is_contiguous():
+        raise ValueError("tokens must be a contiguous 1-D int32 or int64 tensor")
+    return _BITS[tokens.dtype]
+
+
+def embed_fwd(tokens, table, scale: float = 1.0, out=None):
+    """x [T, D] = scale * table[tokens], table [V, D] fp32 or bf16 (formed in
+    fp32, rounded once to the table's type)."""
+    bits = _tokens(tokens)
+    _check_cuda("table", table, tokens.device)
+    dt = _dtype("table", table)
+    if table.dim() != 2 or not table.is_contiguous() or table.shape[0] < 1 or table.shape[1] < 1:
+        raise ValueError("table must be a contiguous [V, D] tensor, V and D at least 1")
+    T, (V, D) = tokens.shape[0], table.shape
+    if out is None:
+        out = torch.empty(T, D, device=table.device, dtype=table.dtype)
+    else:
+        _check_cuda("out", out, table.device)
+        if out.shape != (T, D) or out.dtype != table.dtype or not out.is_contiguous():
+            raise ValueError("out must be a contiguous [T, D] tensor of the table's type")
+    _launch(table.device, lambda: _native.attn_lib().agpt_embed_fwd(
+        _ptr(table), _ptr(tokens), bits, C.c_float(scale), _ptr(out), T, V, D, dt, _stream(table)))
+    return out
+
+
+class EmbedPlan:
+    """The rows of a batch sorted by token, for the gradient of every pass over
+    it: hold one where the tokens stay the same from step to step (the batches
+    of a trie), as TrieAttention.plan is held."""
+
+    def __init__(self, tokens, vocab: int):
+        bits = _tokens(tokens)
+        self.T, self.vocab, self.device = tokens.shape[0], int(vocab), tokens.device
+        lib = _native.attn_lib()
+        if self.vocab < 1:
+            raise ValueError("vocab must be at least 1")
+        self.rows = torch.empty(lib.agpt_embed_plan_ints(self.T, self.vocab), device=self.device, dtype=torch.int32)
+        n = lib.agpt_embed_plan_workspace_bytes(self.T, self.vocab)
+        ws = torch.empty(n, device=self.device, dtype=torch.uint8)
+        _launch(self.device, lambda: lib.agpt_embed_plan(
+            _ptr(tokens), bits, self.T, self.vocab, _ptr(self.rows), _ptr(ws), n, _stream(tokens)))
+
+
+def embed_bwd(dx, tokens, vocab: int | None = None, scale: float = 1.0, out=None):
+    """d_table [V, D] fp32 = scale * the sum of dx's rows by token. tokens: the
+    batch's tokens (sorted in this call; vocab needed) or its EmbedPlan. dx
+    [T, D] fp32 or bf16; rows may be strided."""
+    if not isinstance(tokens, EmbedPlan):
+        if vocab is None:
+            raise ValueError("vocab is needed with tokens that are not planned")
+        tokens = EmbedPlan(tokens, vocab)
+    elif vocab is not None and vocab != tokens.vocab:
+        raise ValueError("the plan has another vocabulary")
+    plan = tokens
+    _check_cuda("dx", dx, plan.device)
+    dt, ld = _dtype("dx", dx), _rows("dx", dx)
+    T, D = dx.shape
+    if T != plan.T or D < 1:
+        raise ValueError("dx must have one row per token, at least one wide")
+    if out is None:
+        out = torch.empty(plan.vocab, D, device=dx.device, dtype=torch.float32)
+    else:
+        _check_cuda("out", out, dx.device)
+        if out.shape != (plan.vocab, D) or out.dtype != torch.float32 or not out.is_contiguous():
+            raise ValueError("out must be a contiguous float32 [vocab, D] tensor")
+    lib = _native.attn_lib()
+    n = lib.agpt_embed_bwd_workspace_floats(T, D)
+    ws = torch.empty(n, device=dx.device, dtype=torch.float32)
+    _launch(dx.device, lambda: lib.agpt_embed_bwd(
+        _ptr(dx), ld, _ptr(plan.rows), C.c_float(scale), _ptr(out), _ptr(ws), n, T, plan.vocab, D, dt, _stream(dx)))
+    return out

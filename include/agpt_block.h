@@ -40,6 +40,39 @@ int agpt_bias_rope_split(const float* qkv, const float* bias, const int32_t* pos
                          const float* cos_t, const float* sin_t, int rope_seq_len, int64_t T,
                          int n_heads, int head_dim, float* q, float* k, float* v, void* stream);
 
+/* The split with a norm of every query and key head in front of the rotation.
+ * qkv [T, (n_heads + 2 n_kv_heads) * head_dim] of `dtype` (AGPT_DTYPE_*), row
+ * stride ld_qkv elements, holds the q | k | v column blocks of one GEMM (n_heads
+ * query heads; n_kv_heads key and value heads). Per head of q and k, with
+ * u = qkv + bias (bias fp32 over the row, NULL = none):
+ *     y = u * w / sqrt(mean(u^2) + eps),   w = wq or wk [head_dim] fp32,
+ * then, when cos_t is not NULL, the rotation of agpt_bias_rope at positions[t].
+ * v is u. Writes contiguous q [T, n_heads * head_dim] and k, v
+ * [T, n_kv_heads * head_dim] of `dtype`, rounded once. head_dim a multiple of 4
+ * from 4 to 256; all buffers (positions apart) 16-byte aligned, ld_qkv a
+ * multiple of 4 elements (of 8 in bf16 where head_dim is); outputs must not overlap inputs. One pass over qkv. The
+ * reference has no norm of queries and keys. */
+int agpt_qk_norm_rope_split(const void* qkv, int64_t ld_qkv, const float* bias, const float* wq, const float* wk,
+                            const int32_t* positions, const float* cos_t, const float* sin_t, int rope_seq_len,
+                            int64_t T, int n_heads, int n_kv_heads, int head_dim, float eps, int dtype, void* q,
+                            void* k, void* v, void* stream);
+
+/* Its backward from dq, dk, dv (contiguous, of `dtype`; gradients of the
+ * outputs) and the forward's qkv, bias, weights and tables. cos_t NULL: dq and
+ * dk are gradients in front of the rotation already (as agpt_attn_bwd returns
+ * them when it is given the tables). Writes dqkv (row stride ld_dqkv), and in
+ * fp32 dwq, dwk [head_dim] and, when dbias is not NULL, dbias over the row:
+ * sums over rows in a fixed order (per-workgroup partials in `workspace`, at
+ * least agpt_qk_norm_workspace_floats floats, then a fold), so two calls give
+ * identical bytes. T = 0 gives zero sums. */
+int agpt_qk_norm_rope_split_bwd(const void* dq, const void* dk, const void* dv, const void* qkv, int64_t ld_qkv,
+                                const float* bias, const float* wq, const float* wk, const int32_t* positions,
+                                const float* cos_t, const float* sin_t, int rope_seq_len, int64_t T, int n_heads,
+                                int n_kv_heads, int head_dim, float eps, int dtype, void* dqkv, int64_t ld_dqkv,
+                                float* dwq, float* dwk, float* dbias, float* workspace, int64_t workspace_floats,
+                                void* stream);
+int64_t agpt_qk_norm_workspace_floats(int n_heads, int n_kv_heads, int head_dim);
+
 /* RMSProp without momentum over n fp32 parameters:
  *     s = beta s + (1 - beta) g^2,   p -= lr g / (sqrt(s) + eps).
  * Replaces cuda_rmsprop_bulk (the µGPT extern of agpt_train.cu:69, called at
