@@ -8,6 +8,21 @@ output projection, the per-query AGPT loss (sum over queries), and an RMSProp
 update of every parameter (one flat fp32 buffer, as the reference's
 d_weights). X = tok_emb[token]; positions enter through RoPE at depth - 1.
 
+Options that the reference does not have (all off by default):
+  embed="lookup"  X = emb_scale * tok_emb[token] by lookup, its gradient by
+                  sorted tokens on a plan held per batch (agpt_amd.embed)
+                  instead of products with one-hot rows
+  qk_norm=True    an RMSNorm of every query and key head in front of RoPE,
+                  in the projection epilogue (weights qn_w, kn_w [head_dim])
+  act8=True       the inputs of the q|k|v, feed-forward and output
+                  projections kept in 8 bits for the backward
+                  (agpt_amd.act8): per row and layer 0.8 KB instead of 3 KB
+                  at d_model 128, d_ff 512. The forward is unchanged; weight
+                  gradients are formed from the kept values, whose distance
+                  from the activations is at most half a step of 1/127 .. 2/127
+                  of the largest in their block of 32; dx, biases and the
+                  ReLU's mask are exact
+
 Native (libagpt_attn.so): trie attention fwd/bwd, the bias + RoPE epilogue,
 the row norms, the loss and RMSProp. The plain GEMMs are torch's
 (hipBLASLt), ReLU and the residual adds torch's elementwise kernels; torch
@@ -24,7 +39,7 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
-from . import block, loss as L
+from . import act8, block, embed, loss as L
 from .attention import TrieAttention, rope_tables
 
 
@@ -38,6 +53,10 @@ class ModelConfig:
     max_depth: int = 32
     norm: str = "rms"
     eps: float = 1e-5
+    embed: str = "onehot"
+    emb_scale: float = 1.0
+    qk_norm: bool = False
+    act8: bool = False
 
 
 def param_shapes(cfg: ModelConfig) -> list[tuple[str, tuple[int, ...]]]:
@@ -48,8 +67,10 @@ def param_shapes(cfg: ModelConfig) -> list[tuple[str, tuple[int, ...]]]:
         # wq, wk, wv (and bq, bk, bv) adjacent: one [3D, D] projection
         out += [(f"n1_w{l}", (D,)), (f"n1_b{l}", (D,)),
                 (f"wq{l}", (D, D)), (f"wk{l}", (D, D)), (f"wv{l}", (D, D)),
-                (f"bq{l}", (D,)), (f"bk{l}", (D,)), (f"bv{l}", (D,)), (f"wo{l}", (D, D)), (f"bo{l}", (D,)),
-                (f"n2_w{l}", (D,)), (f"n2_b{l}", (D,)),
+                (f"bq{l}", (D,)), (f"bk{l}", (D,)), (f"bv{l}", (D,)), (f"wo{l}", (D, D)), (f"bo{l}", (D,))]
+        if cfg.qk_norm:
+            out += [(f"qn_w{l}", (D // cfg.n_heads,)), (f"kn_w{l}", (D // cfg.n_heads,))]
+        out += [(f"n2_w{l}", (D,)), (f"n2_b{l}", (D,)),
                 (f"w1{l}", (Fd, D)), (f"b1{l}", (Fd,)), (f"w2{l}", (D, Fd)), (f"b2{l}", (D,))]
     out += [("nf_w", (D,)), ("nf_b", (D,)), ("w_out", (V, D)), ("b_out", (V,))]
     return out
@@ -62,7 +83,7 @@ def init_params(cfg: ModelConfig, seed: int = 0) -> np.ndarray:
     parts = []
     for name, shape in param_shapes(cfg):
         n = int(np.prod(shape))
-        if name.startswith(("n1_w", "n2_w", "nf_w")):
+        if name.startswith(("n1_w", "n2_w", "nf_w", "qn_w", "kn_w")):
             parts.append(np.ones(n, np.float32))
         elif name.startswith(("b", "n1_b", "n2_b", "nf_b")) or name in ("b_out",):
             parts.append(np.zeros(n, np.float32))
@@ -142,6 +163,7 @@ class TrieBatch:
         if int(token.max(initial=0)) >= cfg.vocab:
             raise ValueError("trie tokens exceed the model vocabulary")
         self.tokens = torch.from_numpy(token.astype(np.int64)).to(dev)
+        self.embed_plan = embed.EmbedPlan(self.tokens, cfg.vocab) if cfg.embed == "lookup" else None
         self.positions = torch.from_numpy((depth - 1).astype(np.int32)).to(dev)
         R = qoff.shape[0] - 1
         edge_len = np.diff(qoff).astype(np.int32)
@@ -156,29 +178,61 @@ class TrieBatch:
         self.loss_args = [to(q2n), to(qoff), to(rid), to(token), to(coff), to(ctok), to(cval)]
 
 
+class _Kept:
+    """A linear layer's input as its backward keeps it: the tensor itself, or an
+    8-bit checkpoint. `tensors` go through save_for_backward."""
+
+    def __init__(self, x, bits8: bool, relu: bool = False):
+        k = act8.pack(x, relu=relu) if bits8 else None
+        self.tensors = (k.codes, k.scales) if bits8 else (x,)
+        self.shape = (k.T, k.W, k.relu) if bits8 else None
+
+    def act(self, tensors) -> act8.Act8:
+        return act8.Act8(*tensors, *self.shape)
+
+    def wgrad(self, tensors, dy, bias: bool):
+        """(dw, db or None) of the layer from the saved tensors."""
+        if self.shape is not None:
+            return act8.wgrad(dy, self.act(tensors), bias)
+        db = None
+        if bias:
+            db = _col_sum(dy) if dy.shape[1] < 128 else dy.sum(0)
+        return _wgrad(dy, tensors[0]), db
+
+
 class _QKVAttn(torch.autograd.Function):
     """x -> fused Q|K|V projection x·Wᵀ ([T, 3D]) -> bias + RoPE epilogue ->
     trie attention. The backward writes dq, dk, dv (pre-RoPE, i.e. gradients
     of the projection's output before its bias) into one [3, T, D] buffer and
     forms dx as three accumulating products dq·Wq + dk·Wk + dv·Wv, so the
-    three gradients are never concatenated into [T, 3D]."""
+    three gradients are never concatenated into [T, 3D]. With a norm of queries
+    and keys (wqn given) its backward writes the [T, 3D] gradient itself."""
 
     @staticmethod
-    def forward(ctx, x, w, b, m, grp):
+    def forward(ctx, x, w, b, wqn, wkn, m, grp):
         att, batch = grp
         qkv = F.linear(x, w)
-        q, k, v = block.bias_rope_split(qkv, b.detach(), batch.positions, m.cos, m.sin, m.cfg.n_heads)
+        H = m.cfg.n_heads
+        if wqn is None:
+            q, k, v = block.bias_rope_split(qkv, b.detach(), batch.positions, m.cos, m.sin, H)
+            norm = ()
+        else:
+            q, k, v = block.qk_norm_rope_split(qkv, wqn.detach(), wkn.detach(), b.detach(), batch.positions, m.cos, m.sin,
+                                               H, eps=m.cfg.eps)
+            norm = (qkv, b, wqn, wkn)
         del qkv
         m._hook()
         o, lse = att.forward(q, k, v)
         m._hook()
-        ctx.save_for_backward(x, w, q, k, v, o, lse)
-        ctx.m, ctx.att = m, att
+        ctx.x = _Kept(x, m.cfg.act8)
+        ctx.save_for_backward(w, q, k, v, o, lse, *ctx.x.tensors, *norm)
+        ctx.m, ctx.att, ctx.n_norm = m, att, len(norm)
         return o
 
     @staticmethod
     def backward(ctx, d_o):
-        x, w, q, k, v, o, lse = ctx.saved_tensors
+        w, q, k, v, o, lse, *rest = ctx.saved_tensors
+        x, norm = rest[:len(rest) - ctx.n_norm], rest[len(rest) - ctx.n_norm:]
         m = ctx.m
         T, D = q.shape
         d3 = torch.empty(3, T, D, device=q.device, dtype=q.dtype)
@@ -186,15 +240,24 @@ class _QKVAttn(torch.autograd.Function):
         ctx.att.backward(q, k, v, o, lse, d_o.contiguous(), rope=(m.cos, m.sin), out=(d3[0], d3[1], d3[2]))
         m._hook()
         w = w.detach()
+        if norm:
+            qkv, b, wqn, wkn = (t.detach() for t in norm)
+            dqkv, dwq, dwk, db = block.qk_norm_rope_split_bwd(d3[0], d3[1], d3[2], qkv, wqn, wkn, b,
+                                                              n_heads=m.cfg.n_heads, eps=m.cfg.eps)
+            del d3
+            return dqkv @ w, ctx.x.wgrad(x, dqkv, False)[0], db, dwq, dwk, None, None
         dx = d3[0] @ w[:D]
         dx.addmm_(d3[1], w[D:2 * D])
         dx.addmm_(d3[2], w[2 * D:])
-        dw = torch.cat([_wgrad(d3[j], x) for j in range(3)])
+        grads = [ctx.x.wgrad(x, d3[j], m.cfg.act8) for j in range(3)]
+        dw = torch.cat([g[0] for g in grads])
+        if m.cfg.act8:
+            return dx, dw, torch.cat([g[1] for g in grads]), None, None, None, None
         # The bias gradient as matrix-vector products (a column sum over ~1M
         # rows as a plain reduction keeps only D outputs in flight).
         ones = torch.ones(1, T, device=q.device, dtype=q.dtype)
         db = torch.matmul(ones, d3).view(3 * D)
-        return dx, dw, db, None, None
+        return dx, dw, db, None, None, None, None
 
 
 def _col_sum(dy: torch.Tensor, rows: int = 64) -> torch.Tensor:
@@ -224,21 +287,20 @@ def _wgrad(dy: torch.Tensor, x: torch.Tensor, splits: int = 64) -> torch.Tensor:
 class _Lin(torch.autograd.Function):
     """x·Wᵀ (+ b, hipBLASLt's fused bias epilogue). Backward: dx = dy·W, the
     weight gradient by _wgrad, the bias gradient by _col_sum when the output
-    is narrow (the vocabulary) and a plain column sum otherwise."""
+    is narrow (the vocabulary) and a plain column sum otherwise; with bits8
+    both by act8.wgrad from the checkpointed x."""
 
     @staticmethod
-    def forward(ctx, x, w, b):
-        ctx.save_for_backward(x, w)
+    def forward(ctx, x, w, b, bits8=False):
+        ctx.x = _Kept(x, bits8)
+        ctx.save_for_backward(w, *ctx.x.tensors)
         ctx.has_b = b is not None
         return F.linear(x, w, b)
 
     @staticmethod
     def backward(ctx, dy):
-        x, w = ctx.saved_tensors
-        db = None
-        if ctx.has_b:
-            db = _col_sum(dy) if dy.shape[1] < 128 else dy.sum(0)
-        return dy @ w, _wgrad(dy, x), db
+        w, *x = ctx.saved_tensors
+        return dy @ w, *ctx.x.wgrad(x, dy, ctx.has_b), None
 
 
 class _LinRelu(torch.autograd.Function):
@@ -257,6 +319,43 @@ class _LinRelu(torch.autograd.Function):
         x, w, h = ctx.saved_tensors
         dh, db = block.relu_bwd(dy.contiguous(), h)
         return dh @ w, _wgrad(dh, x), db
+
+
+class _FFN8(torch.autograd.Function):
+    """W2·relu(W1·x + b1) + b2 with both layers' inputs kept in 8 bits. The
+    backward's pass between the two layers masks the ReLU's gradient and forms
+    W1's and b1's (act8.relu_wgrad)."""
+
+    @staticmethod
+    def forward(ctx, x, w1, b1, w2, b2, hook):
+        h = torch._addmm_activation(b1, x, w1.t(), use_gelu=False)
+        if hook is not None:
+            hook(h)
+        ctx.x, ctx.h = _Kept(x, True), _Kept(h, True, relu=True)
+        ctx.save_for_backward(w1, w2, *ctx.x.tensors, *ctx.h.tensors)
+        return F.linear(h, w2, b2)
+
+    @staticmethod
+    def backward(ctx, dy):
+        w1, w2, xc, xs, hc, hs = ctx.saved_tensors
+        dy = dy.contiguous()
+        h = ctx.h.act((hc, hs))
+        dw2, db2 = act8.wgrad(dy, h)
+        dh, dw1, db1 = act8.relu_wgrad(dy @ w2, h, ctx.x.act((xc, xs)))
+        return dh @ w1, dw1, db1, dw2, db2, None
+
+
+class _Lookup(torch.autograd.Function):
+    """X = scale·E[token] by lookup; dE by sorted tokens on the batch's plan."""
+
+    @staticmethod
+    def forward(ctx, emb, batch, scale):
+        ctx.plan, ctx.scale = batch.embed_plan, scale
+        return embed.embed_fwd(batch.tokens, emb.detach(), scale)
+
+    @staticmethod
+    def backward(ctx, dx):
+        return embed.embed_bwd(dx.contiguous(), ctx.plan, scale=ctx.scale), None, None
 
 
 class _Embed(torch.autograd.Function):
@@ -338,6 +437,10 @@ class TrieGPT:
                  beta: float = 0.999, eps: float = 1e-8):
         if cfg.d_model not in (64, 128, 256, 512) or cfg.d_ff not in (64, 128, 256, 512):
             raise ValueError("the native row kernels take d_model and d_ff of 64, 128, 256 or 512")
+        if cfg.embed not in ("onehot", "lookup"):
+            raise ValueError('embed must be "onehot" or "lookup"')
+        if cfg.emb_scale != 1.0 and cfg.embed != "lookup":
+            raise ValueError('emb_scale needs embed="lookup"')
         self.cfg = cfg
         self.dev = torch.device(device)
         self.flat = torch.from_numpy(init_params(cfg, seed)).to(self.dev).requires_grad_(True)
@@ -418,19 +521,26 @@ class TrieGPT:
         batch = grp[1]
         # X = onehot(token) · tok_emb: the backward is a product onehotᵀ · dX
         # (the gather's backward would scatter-add 1M rows into 65).
-        x = _Embed.apply(batch.tokens, P["tok_emb"])
+        if cfg.embed == "lookup":
+            x = _Lookup.apply(P["tok_emb"], batch, cfg.emb_scale)
+        else:
+            x = _Embed.apply(batch.tokens, P["tok_emb"])
         for l in range(cfg.n_layers):
             # x feeds the norm and the residual add: _NormRes passes it on so
             # both gradients meet inside the norm backward.
             n1, x = self._norm_res(x, P[f"n1_w{l}"], P[f"n1_b{l}"])
-            o = _QKVAttn.apply(n1, P[f"wqkv{l}"], P[f"bqkv{l}"], self, grp)
+            o = _QKVAttn.apply(n1, P[f"wqkv{l}"], P[f"bqkv{l}"], P.get(f"qn_w{l}"), P.get(f"kn_w{l}"), self, grp)
             x = x + _Lin.apply(o, P[f"wo{l}"], P[f"bo{l}"])
             n2, x = self._norm_res(x, P[f"n2_w{l}"], P[f"n2_b{l}"])
+            if cfg.act8:
+                hook = None if self.relu_hook is None else (lambda h, l=l: self.relu_hook(l, h))
+                x = x + _FFN8.apply(n2, P[f"w1{l}"], P[f"b1{l}"], P[f"w2{l}"], P[f"b2{l}"], hook)
+                continue
             h = _LinRelu.apply(n2, P[f"w1{l}"], P[f"b1{l}"])
             if self.relu_hook is not None:
                 self.relu_hook(l, h)
             x = x + _Lin.apply(h, P[f"w2{l}"], P[f"b2{l}"])
-        logits = _Lin.apply(self._norm(x, P["nf_w"], P["nf_b"]), P["w_out"], P["b_out"])
+        logits = _Lin.apply(self._norm(x, P["nf_w"], P["nf_b"]), P["w_out"], P["b_out"], cfg.act8)
         return _Loss.apply(logits, batch)
 
     def step(self) -> torch.Tensor:
@@ -448,14 +558,21 @@ class TrieGPT:
                 block.rmsprop_(self.flat.data, self.flat.grad, self.sq_avg, self.lr, self.beta, self.eps)
         return total
 
+    def _mgpt(self) -> None:
+        """An MGPT file has no place for the norms' weights or the scale."""
+        if self.cfg.qk_norm or self.cfg.emb_scale != 1.0:
+            raise ValueError("MGPT checkpoints hold no query / key norms and no embedding scale")
+
     def save(self, path: str) -> None:
         """Writes the parameters as an MGPT checkpoint (agpt_train.cu:1262-1296)."""
         from .checkpoint import save_mgpt
+        self._mgpt()
         save_mgpt(path, self.cfg, self.flat.detach().cpu().numpy())
 
     def load(self, path: str) -> None:
         """Reads an MGPT checkpoint of this model's shape into the parameters."""
         from .checkpoint import load_mgpt
+        self._mgpt()
         cfg, flat = load_mgpt(path, norm=self.cfg.norm)
         if (cfg.vocab, cfg.d_model, cfg.n_heads, cfg.n_layers, cfg.d_ff) != (
                 self.cfg.vocab, self.cfg.d_model, self.cfg.n_heads, self.cfg.n_layers, self.cfg.d_ff):

@@ -464,7 +464,9 @@ def bench_c3(args) -> int:
     dev = torch.device("cuda:0")
     log(f"building C1 trie with counts (scale {args.scale})")
     tr = trie_mod.config_trie("C1", args.scale, counts=True)
-    cfg = model.ModelConfig(vocab=65, d_model=128, n_heads=8, n_layers=4, d_ff=512, max_depth=32, norm="rms")
+    opts = {k: v for k, v in (("embed", "lookup" if args.c3_lookup else None), ("qk_norm", args.c3_qk_norm),
+                              ("act8", args.c3_act8)) if v}
+    cfg = model.ModelConfig(vocab=65, d_model=128, n_heads=8, n_layers=4, d_ff=512, max_depth=32, norm="rms", **opts)
     m = model.TrieGPT(cfg, device=dev, seed=1)
     m.plan(tr, max_rows=1 << 20)
     log(f"C3: {tr.n_nodes} node-tokens in {len(m.groups)} batches; {m.flat.numel()} parameters")
@@ -494,6 +496,8 @@ def bench_c3(args) -> int:
     m.attn_hook = None
     ms = float(np.mean(step_ms))
     am = float(np.mean(attn_ms))
+    peak = torch.cuda.max_memory_allocated(dev) / 2**30
+    log(f"C3 peak memory {peak:.2f} GiB, options {opts}")
     log(f"C3 step {ms:.2f} ms, trie attention {am:.2f} ms ({am / ms:.1%}); loss {losses[0]:.4g} -> {losses[-1]:.4g}")
     out = {
         "metric": C3_METRIC, "value": tr.n_nodes * 1e3 / ms, "unit": "node-tokens/s", "n_gpus": 1,
@@ -503,7 +507,8 @@ def bench_c3(args) -> int:
         "config": {"workload": "C3: 4-layer training step on the C1 trie", "node_tokens": tr.n_nodes,
                    "batches": len(m.groups), "d_model": 128, "heads": 8, "layers": 4, "d_ff": 512,
                    "vocab": 65, "norm": "rms", "optimizer": "rmsprop(beta=0.999, lr=3e-4)",
-                   "loss": "per-query AGPT loss, linear mass weights"},
+                   "loss": "per-query AGPT loss, linear mass weights", **opts},
+        "peak_memory_GiB": peak,
         "attention_ms_per_step": am, "attention_share": am / ms,
         "loss_first_last": [losses[0], losses[-1]],
         "cpu_baseline": None,
@@ -692,6 +697,10 @@ def main() -> int:
                     help="attn: trie attention fwd+bwd (the headline); loss: per-query AGPT loss; "
                          "c3: the 4-layer training step of config C3 (C1 trie); varlen: the packed "
                          "varlen drop-ins a renaming caller gets (fp32 workloads)")
+    ap.add_argument("--c3-lookup", action="store_true",
+                    help="c3 path: the embedding by lookup, its gradient by sorted tokens")
+    ap.add_argument("--c3-qk-norm", action="store_true", help="c3 path: norms of query and key heads")
+    ap.add_argument("--c3-act8", action="store_true", help="c3 path: linear layers' inputs kept in 8 bits")
     ap.add_argument("--vocab", type=int, default=65, help="loss path: vocabulary size V")
     ap.add_argument("--varlen-layout", default="node", choices=["node", "radix"],
                     help="varlen path: one query per node (agpt_varlen_attention) or the queries of "
