@@ -195,7 +195,10 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(const T* __restrict_
                                                             float* __restrict__ dw, float* __restrict__ db,
                                                             int64_t db_ld, Grad g) {
   const int lane = thread_x() & 63, l = lane & 31, half = lane >> 5;
-  const int64_t unit = static_cast<int64_t>(block_x()) * (kThreads / 64) + (thread_x() >> 6);
+  // the wave's number is one for all its lanes: its rows' addresses are scalar,
+  // and a lane adds one 32-bit offset that stays the same for every step
+  const int wave = __builtin_amdgcn_readfirstlane(thread_x() >> 6);
+  const int64_t unit = static_cast<int64_t>(block_x()) * (kThreads / 64) + wave;
   const int tiles = g.tiles_o * g.tiles_i;
   const int chunk = static_cast<int>(unit / tiles), tile = static_cast<int>(unit - static_cast<int64_t>(chunk) * tiles);
   if (chunk >= g.chunks) return;
@@ -207,6 +210,12 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(const T* __restrict_
   const int quads = g.in / 4, quad = i0 / 4 + l;
   const bool inq = quad < quads;
   const int64_t blocks = (g.rows + kRows - 1) / kRows;
+  const uint32_t off_a = static_cast<uint32_t>(half * kRows * g.ld + oa) * sizeof(T);
+  const uint32_t off_b = static_cast<uint32_t>(half * kRows * g.ld + ob) * sizeof(T);
+  const uint32_t off_d = static_cast<uint32_t>(half * kRows * g.out + oa) * sizeof(T);
+  const uint32_t off_c = static_cast<uint32_t>(half * quads + quad) * (4 * kRows);
+  const uint32_t off_s = static_cast<uint32_t>(half * (quads / 8) + quad / 8) * kRows;
+  const uint32_t off_h = static_cast<uint32_t>(half * (g.out / 4) + oa / 4) * (4 * kRows);
 
   f32x16 acc[2][4];
 #pragma unroll
@@ -218,51 +227,59 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(const T* __restrict_
   float sum_a = 0.0f, sum_b = 0.0f;
   const bool sums = db != nullptr && ti == 0, writes = kRelu && ti == 0;
 
-  auto load = [&](int64_t t, Raw<T>& w) {
-    const int64_t first = t + half * kRows;
-    const int64_t rb = first / kRows;
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      const bool row = first + r < t1;
-      const T* p = dy + (first + r) * g.ld;
-      if constexpr (sizeof(T) == 4) {
-        w.a[r][0] = w.a[r][1] = 0u;
-        if constexpr (kPair) {
-          if (row && ina) {
-            const uint2 v = *reinterpret_cast<const uint2*>(p + oa);
-            w.a[r][0] = v.x;
-            w.a[r][1] = v.y;
-          }
-        } else {
-          if (row && ina) w.a[r][0] = __float_as_uint(p[oa]);
-          if (row && inb) w.a[r][1] = __float_as_uint(p[ob]);
+  auto row = [&](const char* p, Raw<T>& w, int r, bool a, bool b) {
+    if constexpr (sizeof(T) == 4) {
+      w.a[r][0] = w.a[r][1] = 0u;
+      if constexpr (kPair) {
+        if (a) {
+          const uint2 v = *reinterpret_cast<const uint2*>(p + off_a);
+          w.a[r][0] = v.x;
+          w.a[r][1] = v.y;
         }
       } else {
-        w.a[r][0] = 0u;
-        if constexpr (kPair) {
-          if (row && ina) w.a[r][0] = *reinterpret_cast<const uint32_t*>(p + oa);
-        } else {
-          if (row && ina) w.a[r][0] = p[oa].bits;
-          if (row && inb) w.a[r][0] |= static_cast<uint32_t>(p[ob].bits) << 16;
-        }
+        if (a) w.a[r][0] = *reinterpret_cast<const uint32_t*>(p + off_a);
+        if (b) w.a[r][1] = *reinterpret_cast<const uint32_t*>(p + off_b);
+      }
+    } else {
+      w.a[r][0] = 0u;
+      if constexpr (kPair) {
+        if (a) w.a[r][0] = *reinterpret_cast<const uint32_t*>(p + off_a);
+      } else {
+        if (a) w.a[r][0] = *reinterpret_cast<const uint16_t*>(p + off_a);
+        if (b) w.a[r][0] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + off_b)) << 16;
       }
     }
-    // no block of the checkpoint, or no such columns: scale 0, value 0
-    const bool live = inq && rb < blocks;
+  };
+  auto load = [&](int64_t t, Raw<T>& w) {
+    const char* p = reinterpret_cast<const char*>(dy + t * g.ld);
+    const int64_t step = g.ld * static_cast<int64_t>(sizeof(T)), rb = t / kRows;
+    const bool whole = t + kStep <= t1;
+    if (whole) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) row(p + r * step, w, r, ina, inb);
+    } else {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const bool in = t + half * kRows + r < t1;
+        row(p + r * step, w, r, in && ina, in && inb);
+      }
+    }
+    // no such columns, or no block of the checkpoint: scale 0, value 0
+    const bool live = whole || rb + half < blocks;
     w.c0 = w.c1 = uint4{0u, 0u, 0u, 0u};
     w.sc = uint2{0u, 0u};
-    if (live) {
-      const uint4* c = reinterpret_cast<const uint4*>(codes + (rb * quads + quad) * (4 * kRows));
-      w.c0 = c[0];
-      w.c1 = c[1];
-      w.sc = *reinterpret_cast<const uint2*>(scales + (rb * (quads / 8) + quad / 8) * kRows);
+    if (live && inq) {
+      const char* c = reinterpret_cast<const char*>(codes) + rb * quads * (4 * kRows);
+      w.c0 = *reinterpret_cast<const uint4*>(c + off_c);
+      w.c1 = *reinterpret_cast<const uint4*>(c + off_c + 16);
+      w.sc = *reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(scales) + rb * (quads / 8) * kRows + off_s);
     }
     if constexpr (kRelu) {
       w.h0 = w.h1 = uint4{0u, 0u, 0u, 0u};
-      if (ina && rb < blocks) {
-        const uint4* c = reinterpret_cast<const uint4*>(hc + (rb * (g.out / 4) + oa / 4) * (4 * kRows));
-        w.h0 = c[0];
-        w.h1 = c[1];
+      if (live && ina) {
+        const char* c = reinterpret_cast<const char*>(hc) + rb * (g.out / 4) * (4 * kRows);
+        w.h0 = *reinterpret_cast<const uint4*>(c + off_h);
+        w.h1 = *reinterpret_cast<const uint4*>(c + off_h + 16);
       }
     }
   };
@@ -280,10 +297,17 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(const T* __restrict_
         } else {
           w.a[r][0] &= ((m & 0xffu) ? 0xffffu : 0u) | ((m & 0xff00u) ? 0xffff0000u : 0u);
         }
-        if (writes && ina && t + half * kRows + r < t1) {
-          T* p = dh + (t + half * kRows + r) * g.out + oa;
-          if constexpr (sizeof(T) == 4) *reinterpret_cast<uint2*>(p) = uint2{w.a[r][0], w.a[r][1]};
-          else *reinterpret_cast<uint32_t*>(p) = w.a[r][0];
+      }
+      if (writes) {
+        char* p = reinterpret_cast<char*>(dh + t * g.out);
+        const int64_t drow = g.out * static_cast<int64_t>(sizeof(T));
+        const bool whole = t + kStep <= t1;
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          if (ina && (whole || t + half * kRows + r < t1)) {
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint2*>(p + r * drow + off_d) = uint2{w.a[r][0], w.a[r][1]};
+            else *reinterpret_cast<uint32_t*>(p + r * drow + off_d) = w.a[r][0];
+          }
         }
       }
     }
@@ -453,6 +477,7 @@ int wgrad(const char* what, const void* dy, int64_t ld, int dtype, const uint8_t
   if (!aligned(codes, 16) || !aligned(scales, 16) || !aligned(dw, 16) || !aligned(db, 16) || !aligned(ws, 16))
     return invalid(what, "codes, scales, dw, db and workspace must be 16-byte aligned");
   if (!aligned(dy, es)) return invalid(what, "dy is not aligned to its elements");
+  if (ld > (1 << 26)) return agpt_internal_set_error(AGPT_ERR_UNSUPPORTED, "agpt_act8: row strides above 2^26 are not supported");
   const bool pair = out % 2 == 0 && ld % 2 == 0 && aligned(dy, 2 * es);
   const Plan p = plan_of(T, out, in);
   const hipStream_t st = static_cast<hipStream_t>(stream);
