@@ -210,12 +210,15 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(const T* __restrict_
   const int quads = g.in / 4, quad = i0 / 4 + l;
   const bool inq = quad < quads;
   const int64_t blocks = (g.rows + kRows - 1) / kRows;
-  const uint32_t off_a = static_cast<uint32_t>(half * kRows * g.ld + oa) * sizeof(T);
-  const uint32_t off_b = static_cast<uint32_t>(half * kRows * g.ld + ob) * sizeof(T);
-  const uint32_t off_d = static_cast<uint32_t>(half * kRows * g.out + oa) * sizeof(T);
-  const uint32_t off_c = static_cast<uint32_t>(half * quads + quad) * (4 * kRows);
-  const uint32_t off_s = static_cast<uint32_t>(half * (quads / 8) + quad / 8) * kRows;
-  const uint32_t off_h = static_cast<uint32_t>(half * (g.out / 4) + oa / 4) * (4 * kRows);
+  // A column past the edge is read as the last one: it only reaches entries of
+  // dW, db and dh that are not written.
+  const int ca = ina ? oa : g.out - (kPair ? 2 : 1), cb = inb ? ob : g.out - 1, cq = inq ? quad : quads - 1;
+  const uint32_t off_a = static_cast<uint32_t>(half * kRows * g.ld + ca) * sizeof(T);
+  const uint32_t off_b = static_cast<uint32_t>(half * kRows * g.ld + cb) * sizeof(T);
+  const uint32_t off_d = static_cast<uint32_t>(half * kRows * g.out + ca) * sizeof(T);
+  const uint32_t off_c = static_cast<uint32_t>(half * quads + cq) * (4 * kRows);
+  const uint32_t off_s = static_cast<uint32_t>(half * (quads / 8) + cq / 8) * kRows;
+  const uint32_t off_h = static_cast<uint32_t>(half * (g.out / 4) + ca / 4) * (4 * kRows);
 
   f32x16 acc[2][4];
 #pragma unroll
@@ -227,61 +230,52 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(const T* __restrict_
   float sum_a = 0.0f, sum_b = 0.0f;
   const bool sums = db != nullptr && ti == 0, writes = kRelu && ti == 0;
 
-  auto row = [&](const char* p, Raw<T>& w, int r, bool a, bool b) {
-    if constexpr (sizeof(T) == 4) {
-      w.a[r][0] = w.a[r][1] = 0u;
-      if constexpr (kPair) {
-        if (a) {
-          const uint2 v = *reinterpret_cast<const uint2*>(p + off_a);
-          w.a[r][0] = v.x;
-          w.a[r][1] = v.y;
-        }
-      } else {
-        if (a) w.a[r][0] = *reinterpret_cast<const uint32_t*>(p + off_a);
-        if (b) w.a[r][1] = *reinterpret_cast<const uint32_t*>(p + off_b);
-      }
+  auto row = [&](const char* p, Raw<T>& w, int r) {
+    if constexpr (sizeof(T) == 4 && kPair) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p + off_a);
+      w.a[r][0] = v.x;
+      w.a[r][1] = v.y;
+    } else if constexpr (sizeof(T) == 4) {
+      w.a[r][0] = *reinterpret_cast<const uint32_t*>(p + off_a);
+      w.a[r][1] = *reinterpret_cast<const uint32_t*>(p + off_b);
+    } else if constexpr (kPair) {
+      w.a[r][0] = *reinterpret_cast<const uint32_t*>(p + off_a);
     } else {
-      w.a[r][0] = 0u;
-      if constexpr (kPair) {
-        if (a) w.a[r][0] = *reinterpret_cast<const uint32_t*>(p + off_a);
-      } else {
-        if (a) w.a[r][0] = *reinterpret_cast<const uint16_t*>(p + off_a);
-        if (b) w.a[r][0] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + off_b)) << 16;
-      }
+      w.a[r][0] = *reinterpret_cast<const uint16_t*>(p + off_a) |
+                  static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + off_b)) << 16;
     }
   };
   auto load = [&](int64_t t, Raw<T>& w) {
     const char* p = reinterpret_cast<const char*>(dy + t * g.ld);
     const int64_t step = g.ld * static_cast<int64_t>(sizeof(T)), rb = t / kRows;
-    const bool whole = t + kStep <= t1;
-    if (whole) {
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) row(p + r * step, w, r, ina, inb);
-    } else {
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const bool in = t + half * kRows + r < t1;
-        row(p + r * step, w, r, in && ina, in && inb);
+    const char* pc = reinterpret_cast<const char*>(codes) + rb * quads * (4 * kRows);
+    const char* ps = reinterpret_cast<const char*>(scales) + rb * (quads / 8) * kRows;
+    const char* ph = reinterpret_cast<const char*>(hc) + rb * (g.out / 4) * (4 * kRows);
+    auto blocks_of = [&]() {
+      w.c0 = *reinterpret_cast<const uint4*>(pc + off_c);
+      w.c1 = *reinterpret_cast<const uint4*>(pc + off_c + 16);
+      w.sc = *reinterpret_cast<const uint2*>(ps + off_s);
+      if constexpr (kRelu) {
+        w.h0 = *reinterpret_cast<const uint4*>(ph + off_h);
+        w.h1 = *reinterpret_cast<const uint4*>(ph + off_h + 16);
       }
+    };
+    if (t + kStep <= t1) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) row(p + r * step, w, r);
+      blocks_of();
+      return;
     }
-    // no such columns, or no block of the checkpoint: scale 0, value 0
-    const bool live = whole || rb + half < blocks;
-    w.c0 = w.c1 = uint4{0u, 0u, 0u, 0u};
+    // the last step of the last chunk: rows past the end are zeros, and so are the values of a block past it
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+      for (int c = 0; c < (sizeof(T) == 4 ? 2 : 1); ++c) w.a[r][c] = 0u;
+      if (t + half * kRows + r < t1) row(p + r * step, w, r);
+    }
+    w.c0 = w.c1 = w.h0 = w.h1 = uint4{0u, 0u, 0u, 0u};
     w.sc = uint2{0u, 0u};
-    if (live && inq) {
-      const char* c = reinterpret_cast<const char*>(codes) + rb * quads * (4 * kRows);
-      w.c0 = *reinterpret_cast<const uint4*>(c + off_c);
-      w.c1 = *reinterpret_cast<const uint4*>(c + off_c + 16);
-      w.sc = *reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(scales) + rb * (quads / 8) * kRows + off_s);
-    }
-    if constexpr (kRelu) {
-      w.h0 = w.h1 = uint4{0u, 0u, 0u, 0u};
-      if (live && ina) {
-        const char* c = reinterpret_cast<const char*>(hc) + rb * (g.out / 4) * (4 * kRows);
-        w.h0 = *reinterpret_cast<const uint4*>(c + off_h);
-        w.h1 = *reinterpret_cast<const uint4*>(c + off_h + 16);
-      }
-    }
+    if (rb + half < blocks) blocks_of();
   };
 
   auto step = [&](int64_t t, Raw<T>& w) {
@@ -412,6 +406,340 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(const T* __restrict_
   }
 }
 
+// ---- weight gradient, operands shared through LDS ------------------------------------
+// Where dW is wider than a wave's tile, every wave of the kernel above cuts and
+// decodes the same columns again. Here a workgroup of eight waves owns a
+// (64 WO) x (128 WI) tile of dW, WO * WI = 8: per step of 32 rows each wave
+// prepares a share of the operands once, in the lane layout of the matrix
+// instruction, and puts them into LDS; then each wave multiplies its 64 x 128
+// tile out of it. Two LDS buffers: step n is multiplied while step n + 1 is
+// prepared and the rows of step n + 2 are on their way.
+// An operand group is 64 columns: [octet of rows][part][column parity][32 lanes] of 16 bytes
+// (eight rows of a column as bf16), written and read without bank conflicts.
+constexpr int kShared = 512, kSRows = 32, kOctets = kSRows / kRows;
+
+template <typename T, int WO, bool kPair, bool kRelu>
+__global__ __launch_bounds__(kShared, 2) void wgrad_shared_kernel(const T* __restrict__ dy, const uint8_t* __restrict__ hc,
+                                                                  T* __restrict__ dh, const uint8_t* __restrict__ codes,
+                                                                  const uint8_t* __restrict__ scales,
+                                                                  float* __restrict__ dw, float* __restrict__ db,
+                                                                  int64_t db_ld, Grad g, int grid) {
+  constexpr int WI = 8 / WO, kParts = sizeof(T) == 4 ? 3 : 1;
+  constexpr int kGroupA = kOctets * kParts * 2 * 32, kGroupB = kOctets * 2 * 32;  // uint4 each
+  // A wave's jobs of eight rows: of dy with two columns a lane (kPair) or one, of the codes with two.
+  constexpr int kCols = kPair ? 2 : 1, kJobsA = WO / (2 * kCols), kJobsB = WI / 2;
+  __shared__ uint4 sa[2][WO * kGroupA];
+  __shared__ uint4 sb[2][2 * WI * kGroupB];
+  const int lane = thread_x() & 63, l = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(thread_x() >> 6);
+  const int tiles = g.tiles_o * g.tiles_i;
+  // workgroups of one chunk on one XCD (they are dealt over eight in turn), whose L2 then holds the chunk's rows for all of them
+  const int unit = (block_x() & 7) * (grid >> 3) + (block_x() >> 3);
+  const int chunk = unit / tiles, tile = unit - chunk * tiles;
+  if (chunk >= g.chunks) return;
+  const int to = tile / g.tiles_i, ti = tile - to * g.tiles_i;
+  const int o0 = to * 64 * WO, i0 = ti * 128 * WI;
+  const int64_t t0 = chunk * g.chunk_rows, t1 = t0 + g.chunk_rows < g.rows ? t0 + g.chunk_rows : g.rows;
+  const int quads = g.in / 4;
+  const int64_t blocks = (g.rows + kRows - 1) / kRows;
+
+  // This wave's share of the preparation. A column past the edge is read as the
+  // last one: it only reaches entries of dW, db and dh that are not written.
+  int ga[kJobsA], octa[kJobsA], cola[kJobsA];
+  uint32_t off_a[kJobsA], off_d[kJobsA], off_h[kJobsA];
+#pragma unroll
+  for (int q = 0; q < kJobsA; ++q) {
+    const int job = wave * kJobsA + q;
+    ga[q] = kPair ? job >> 1 : job >> 2;
+    octa[q] = kPair ? 2 * (job & 1) + half : job & 3;
+    cola[q] = o0 + 64 * ga[q] + (kPair ? 2 * l : lane);
+    const int c = cola[q] < g.out ? cola[q] : g.out - kCols;
+    off_a[q] = static_cast<uint32_t>(octa[q] * kRows * g.ld + c) * sizeof(T);
+    off_d[q] = static_cast<uint32_t>(octa[q] * kRows * g.out + c) * sizeof(T);
+    off_h[q] = static_cast<uint32_t>(octa[q] * (g.out / 4) + c / 4) * (4 * kRows);
+  }
+  int gb[kJobsB], octb[kJobsB];
+  uint32_t off_c[kJobsB], off_s[kJobsB];
+#pragma unroll
+  for (int q = 0; q < kJobsB; ++q) {
+    gb[q] = kJobsB == 1 ? wave >> 1 : wave;
+    octb[q] = 2 * (kJobsB == 1 ? wave & 1 : q) + half;
+    int quad = (i0 + 64 * gb[q]) / 4 + l / 2;
+    quad = quad < quads ? quad : quads - 1;
+    off_c[q] = static_cast<uint32_t>(octb[q] * quads + quad) * (4 * kRows);
+    off_s[q] = static_cast<uint32_t>(octb[q] * (quads / 8) + quad / 8) * kRows;
+  }
+  const bool sums = db != nullptr && ti == 0, writes = kRelu && ti == 0;
+  float sum[kJobsA][kCols];
+#pragma unroll
+  for (int q = 0; q < kJobsA; ++q)
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) sum[q][c] = 0.0f;
+
+  struct Raw {
+    uint32_t a[kJobsA][kRows][sizeof(T) == 4 ? kCols : 1];
+    uint4 h[kJobsA][2], c[kJobsB][2];
+    uint2 s[kJobsB];
+  };
+  auto load = [&](int64_t t, Raw& w) {
+    const int64_t rb = t / kRows, step = g.ld * static_cast<int64_t>(sizeof(T));
+    const char* pa = reinterpret_cast<const char*>(dy + t * g.ld);
+    const char* pc = reinterpret_cast<const char*>(codes) + rb * quads * (4 * kRows);
+    const char* ps = reinterpret_cast<const char*>(scales) + rb * (quads / 8) * kRows;
+    const char* ph = reinterpret_cast<const char*>(hc) + rb * (g.out / 4) * (4 * kRows);
+    auto row = [&](int q, int r) {
+      const char* p = pa + r * step + off_a[q];
+      if constexpr (sizeof(T) == 4 && kPair) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w.a[q][r][0] = v.x;
+        w.a[q][r][1] = v.y;
+      } else if constexpr (sizeof(T) == 4 || kPair) {
+        w.a[q][r][0] = *reinterpret_cast<const uint32_t*>(p);
+      } else {
+        w.a[q][r][0] = *reinterpret_cast<const uint16_t*>(p);
+      }
+    };
+    auto block_h = [&](int q) {
+      w.h[q][0] = *reinterpret_cast<const uint4*>(ph + off_h[q]);
+      w.h[q][1] = *reinterpret_cast<const uint4*>(ph + off_h[q] + 16);
+    };
+    auto block_c = [&](int q) {
+      w.c[q][0] = *reinterpret_cast<const uint4*>(pc + off_c[q]);
+      w.c[q][1] = *reinterpret_cast<const uint4*>(pc + off_c[q] + 16);
+      w.s[q] = *reinterpret_cast<const uint2*>(ps + off_s[q]);
+    };
+    if (t + kSRows <= t1) {
+#pragma unroll
+      for (int q = 0; q < kJobsA; ++q) {
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) row(q, r);
+        if constexpr (kRelu) block_h(q);
+      }
+#pragma unroll
+      for (int q = 0; q < kJobsB; ++q) block_c(q);
+      return;
+    }
+    // the last step of the last chunk: rows past the end are zeros, and so are the values of blocks past it
+#pragma unroll
+    for (int q = 0; q < kJobsA; ++q) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+        for (int c = 0; c < (sizeof(T) == 4 ? kCols : 1); ++c) w.a[q][r][c] = 0u;
+        if (t + octa[q] * kRows + r < t1) row(q, r);
+      }
+      if constexpr (kRelu) {
+        w.h[q][0] = w.h[q][1] = uint4{0u, 0u, 0u, 0u};
+        if (rb + octa[q] < blocks) block_h(q);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kJobsB; ++q) {
+      w.c[q][0] = w.c[q][1] = uint4{0u, 0u, 0u, 0u};
+      w.s[q] = uint2{0u, 0u};
+      if (rb + octb[q] < blocks) block_c(q);
+    }
+  };
+
+  auto put_a = [&](int64_t t, Raw& w, int q, uint4* to_lds) {
+    auto& ra = w.a[q];
+    if constexpr (kRelu) {
+      const uint32_t h[kRows] = {w.h[q][0].x, w.h[q][0].y, w.h[q][0].z, w.h[q][0].w,
+                                 w.h[q][1].x, w.h[q][1].y, w.h[q][1].z, w.h[q][1].w};
+      const int sh = kPair ? (l & 1) * 16 : (lane & 3) * 8;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const uint32_t m = h[r] >> sh;
+        if constexpr (sizeof(T) == 4 || !kPair) {
+          ra[r][0] = (m & 0xffu) ? ra[r][0] : 0u;
+          if constexpr (kPair) ra[r][1] = (m & 0xff00u) ? ra[r][1] : 0u;
+        } else {
+          ra[r][0] &= ((m & 0xffu) ? 0xffffu : 0u) | ((m & 0xff00u) ? 0xffff0000u : 0u);
+        }
+      }
+      if (writes) {
+        char* p = reinterpret_cast<char*>(dh + t * g.out);
+        const int64_t drow = g.out * static_cast<int64_t>(sizeof(T));
+        const bool whole = t + kSRows <= t1;
+        if (cola[q] < g.out) {
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) {
+            if (whole || t + octa[q] * kRows + r < t1) {
+              char* d = p + r * drow + off_d[q];
+              if constexpr (sizeof(T) == 4 && kPair) *reinterpret_cast<uint2*>(d) = uint2{ra[r][0], ra[r][1]};
+              else if constexpr (sizeof(T) == 4 || kPair) *reinterpret_cast<uint32_t*>(d) = ra[r][0];
+              else *reinterpret_cast<uint16_t*>(d) = static_cast<uint16_t>(ra[r][0]);
+            }
+          }
+        }
+      }
+    }
+    if (sums) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) sum[q][c] += __uint_as_float(ra[r][c]);
+        } else {
+          sum[q][0] += __uint_as_float(ra[r][0] << 16);
+          if constexpr (kPair) sum[q][1] += __uint_as_float(ra[r][0] & 0xffff0000u);
+        }
+      }
+    }
+    uint4* out = to_lds + ga[q] * kGroupA + octa[q] * (kParts * 64) + l;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      const int p = kPair ? c : half;
+      uint32_t m[kRows / 2];
+      if constexpr (sizeof(T) == 4) {
+        float x[kRows];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) x[r] = __uint_as_float(ra[r][c]);
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+#pragma unroll
+          for (int r = 0; r < kRows; r += 2) m[r / 2] = high_pair(__float_as_uint(x[r]), __float_as_uint(x[r + 1]));
+          if (part < 2) {
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) x[r] -= __uint_as_float(__float_as_uint(x[r]) & 0xffff0000u);
+          }
+          out[(part * 2 + p) * 32] = uint4{m[0], m[1], m[2], m[3]};
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < kRows; r += 2)
+          m[r / 2] = c ? high_pair(ra[r][0], ra[r + 1][0]) : low_pair(ra[r][0], ra[r + 1][0]);
+        out[p * 32] = uint4{m[0], m[1], m[2], m[3]};
+      }
+    }
+  };
+  auto put_b = [&](const Raw& w, int q, uint4* to_lds) {
+    const int sh = (l & 1) * 16;
+    const uint32_t c[kRows] = {w.c[q][0].x >> sh, w.c[q][0].y >> sh, w.c[q][0].z >> sh, w.c[q][0].w >> sh,
+                               w.c[q][1].x >> sh, w.c[q][1].y >> sh, w.c[q][1].z >> sh, w.c[q][1].w >> sh};
+    uint32_t v[2][kRows / 2];
+#pragma unroll
+    for (int r = 0; r < kRows; r += 2) {
+      const uint32_t sw = r < 4 ? w.s[q].x : w.s[q].y;
+      const float s0 = scale_of((sw >> (8 * (r % 4))) & 0xffu), z0 = -g.zero * s0;
+      const float s1 = scale_of((sw >> (8 * (r % 4 + 1))) & 0xffu), z1 = -g.zero * s1;
+      v[0][r / 2] = high_pair(__float_as_uint(fmaf(byte_f<0>(c[r]), s0, z0)), __float_as_uint(fmaf(byte_f<0>(c[r + 1]), s1, z1)));
+      v[1][r / 2] = high_pair(__float_as_uint(fmaf(byte_f<1>(c[r]), s0, z0)), __float_as_uint(fmaf(byte_f<1>(c[r + 1]), s1, z1)));
+    }
+    uint4* out = to_lds + gb[q] * kGroupB + octb[q] * 64 + l;
+    out[0] = uint4{v[0][0], v[0][1], v[0][2], v[0][3]};
+    out[32] = uint4{v[1][0], v[1][1], v[1][2], v[1][3]};
+  };
+
+  const int wo = wave / WI, wi = wave - wo * WI;
+  f32x16 acc[2][4];
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[p][j][r] = 0.0f;
+  auto multiply = [&](const uint4* a, const uint4* b) {
+    a += wo * kGroupA + l;
+    b += 2 * wi * kGroupB + l;
+#pragma unroll
+    for (int ks = 0; ks < kOctets / 2; ++ks) {
+      const int oct = 2 * ks + half;
+      uint4 fb[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) fb[j] = b[(j >> 1) * kGroupB + oct * 64 + (j & 1) * 32];
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+          const uint4 fa = a[oct * (kParts * 64) + (part * 2 + p) * 32];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc[p][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fa),
+                                                                __builtin_bit_cast(bf16x8, fb[j]), acc[p][j], 0, 0, 0);
+        }
+    }
+  };
+  auto prepare = [&](int64_t t, Raw& w, int buf) {
+#pragma unroll
+    for (int q = 0; q < kJobsA; ++q) put_a(t, w, q, sa[buf]);
+#pragma unroll
+    for (int q = 0; q < kJobsB; ++q) put_b(w, q, sb[buf]);
+  };
+
+  // Step n is multiplied from buffer n & 1 while step n + 1 is prepared and the
+  // rows of the next kAhead steps are on their way: two where the registers hold
+  // them (64K rows of 1024 x 1000 bf16 208 -> 179 us for one to two), one behind
+  // a ReLU and with two jobs a wave.
+  constexpr int kAhead = kRelu || kJobsA > 1 ? 1 : 2;
+  const int steps = static_cast<int>((t1 - t0 + kSRows - 1) / kSRows);
+  auto at = [&](int n) { return t0 + static_cast<int64_t>(n) * kSRows; };
+  Raw w0, w1;
+  if (steps > 0) load(at(0), w0);
+  if (kAhead == 2 && steps > 1) load(at(1), w1);
+  if (steps > 0) prepare(at(0), w0, 0);
+  if (steps > kAhead) load(at(kAhead), w0);
+  __syncthreads();
+  int n = 0;
+  if constexpr (kAhead == 1) {
+    for (; n < steps; ++n) {
+      const int buf = n & 1;
+      multiply(sa[buf], sb[buf]);
+      if (n + 1 < steps) prepare(at(n + 1), w0, buf ^ 1);
+      if (n + 2 < steps) load(at(n + 2), w0);
+      __syncthreads();
+    }
+  } else {
+    auto body = [&](Raw& w, int buf) {
+      multiply(sa[buf], sb[buf]);
+      prepare(at(n + 1), w, buf ^ 1);
+      if (n + 3 < steps) load(at(n + 3), w);
+      __syncthreads();
+    };
+    while (n + 1 < steps) {
+      body(w1, 0);
+      if (++n + 1 >= steps) break;
+      body(w0, 1);
+      ++n;
+    }
+    if (steps > 0) multiply(sa[n & 1], sb[n & 1]);
+    __syncthreads();
+  }
+
+  float* out = dw + static_cast<int64_t>(chunk) * g.out * g.in;
+#pragma unroll
+  for (int jj = 0; jj < 2; ++jj) {
+    const int i = i0 + 128 * wi + 64 * jj + 2 * l;
+    if (i < g.in) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int m = 8 * (r / 4) + 4 * half + r % 4;
+          const int o = o0 + 64 * wo + (kPair ? 2 * m + p : 32 * p + m);
+          if (o < g.out)
+            *reinterpret_cast<float2*>(out + static_cast<int64_t>(o) * g.in + i) =
+                float2{acc[p][2 * jj][r], acc[p][2 * jj + 1][r]};
+        }
+    }
+  }
+  // db: a column's four octets of rows, added in order (the operands in LDS are no longer needed)
+  if (sums) {
+    float* s = reinterpret_cast<float*>(sa);
+#pragma unroll
+    for (int q = 0; q < kJobsA; ++q)
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) s[octa[q] * (64 * WO) + cola[q] - o0 + c] = sum[q][c];
+    __syncthreads();
+    const int c = thread_x();
+    if (c < 64 * WO && o0 + c < g.out) {
+      float a = s[c];
+      for (int q = 1; q < kOctets; ++q) a += s[q * (64 * WO) + c];
+      db[chunk * db_ld + o0 + c] = a;
+    }
+  }
+}
+
 __global__ __launch_bounds__(kFoldThreads) void wgrad_fold_kernel(const float* __restrict__ part, int64_t n,
                                                                   const float* __restrict__ part_b, int64_t ldb,
                                                                   int chunks, int out, float* __restrict__ dw,
@@ -431,19 +759,27 @@ constexpr int kMinRows = 64;      // of a chunk
 constexpr int kMaxWidth = 32768;
 
 struct Plan {
+  int wo;  // 0: a wave for itself; 2, 4: waves down the shared tile
   int tiles_o, tiles_i, chunks;
   int64_t chunk_rows, db_ld;
 };
-Plan plan_of(int64_t T, int out, int in) {
+// Shared operands where dW is wider than a wave's tile in both directions.
+int shared_wo(int out, int in) {
+  if (out <= kTileO || in <= kTileI) return 0;
+  return out <= 2 * kTileO ? 2 : 4;
+}
+Plan plan_of(int64_t T, int out, int in, int wo) {
   Plan p;
-  p.tiles_o = (out + kTileO - 1) / kTileO;
-  p.tiles_i = (in + kTileI - 1) / kTileI;
+  p.wo = wo;
+  const int to = wo ? 64 * wo : kTileO, ti = wo ? 128 * (8 / wo) : kTileI, step = wo ? kSRows : kStep;
+  p.tiles_o = (out + to - 1) / to;
+  p.tiles_i = (in + ti - 1) / ti;
   const int64_t tiles = static_cast<int64_t>(p.tiles_o) * p.tiles_i;
-  int64_t chunks = kUnits / tiles;
+  int64_t chunks = (wo ? kUnits / 8 : kUnits) / tiles;
   if (chunks > (T + kMinRows - 1) / kMinRows) chunks = (T + kMinRows - 1) / kMinRows;
   if (chunks < 1) chunks = 1;
-  p.chunk_rows = ((T + chunks - 1) / chunks + kStep - 1) / kStep * kStep;
-  if (p.chunk_rows < kStep) p.chunk_rows = kStep;
+  p.chunk_rows = ((T + chunks - 1) / chunks + step - 1) / step * step;
+  if (p.chunk_rows < step) p.chunk_rows = step;
   p.chunks = static_cast<int>((T + p.chunk_rows - 1) / p.chunk_rows);
   if (p.chunks < 1) p.chunks = 1;
   p.db_ld = (out + 3) / 4 * 4;
@@ -479,7 +815,7 @@ int wgrad(const char* what, const void* dy, int64_t ld, int dtype, const uint8_t
   if (!aligned(dy, es)) return invalid(what, "dy is not aligned to its elements");
   if (ld > (1 << 26)) return agpt_internal_set_error(AGPT_ERR_UNSUPPORTED, "agpt_act8: row strides above 2^26 are not supported");
   const bool pair = out % 2 == 0 && ld % 2 == 0 && aligned(dy, 2 * es);
-  const Plan p = plan_of(T, out, in);
+  const Plan p = plan_of(T, out, in, shared_wo(out, in));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t n = static_cast<int64_t>(out) * in;
   const bool direct = p.chunks == 1;
@@ -493,8 +829,22 @@ int wgrad(const char* what, const void* dy, int64_t ld, int dtype, const uint8_t
     hipLaunchKernelGGL((wgrad_kernel<E, decltype(pc)::value, decltype(rc)::value>), grid, dim3(kThreads), 0, st,
                        static_cast<const E*>(dy), hc, static_cast<E*>(dh), codes, scales, part, part_b, p.db_ld, g);
   };
+  auto shared = [&](auto e, auto wc, auto pc, auto rc) {
+    using E = decltype(e);
+    const int n = static_cast<int>((units + 7) / 8 * 8);
+    hipLaunchKernelGGL((wgrad_shared_kernel<E, decltype(wc)::value, decltype(pc)::value, decltype(rc)::value>), dim3(n),
+                       dim3(kShared), 0, st, static_cast<const E*>(dy), hc, static_cast<E*>(dh), codes, scales, part, part_b,
+                       p.db_ld, g, n);
+  };
+  using W2 = std::integral_constant<int, 2>;
+  using W4 = std::integral_constant<int, 4>;
   auto kinds = [&](auto e) {
-    if (hc) go(e, std::true_type{}, std::true_type{});
+    if (p.wo == 2 && hc) shared(e, W2{}, std::false_type{}, std::true_type{});
+    else if (p.wo == 2) shared(e, W2{}, std::false_type{}, std::false_type{});
+    else if (p.wo == 4 && hc) shared(e, W4{}, std::true_type{}, std::true_type{});
+    else if (p.wo == 4 && pair) shared(e, W4{}, std::true_type{}, std::false_type{});
+    else if (p.wo == 4) shared(e, W4{}, std::false_type{}, std::false_type{});
+    else if (hc) go(e, std::true_type{}, std::true_type{});
     else if (pair) go(e, std::true_type{}, std::false_type{});
     else go(e, std::false_type{}, std::false_type{});
   };
@@ -568,7 +918,7 @@ extern "C" int agpt_act8_unpack(const uint8_t* codes, const uint8_t* scales, int
 // One partial dW and db per chunk.
 extern "C" int64_t agpt_act8_wgrad_workspace_floats(int64_t T, int out_width, int in_width) {
   if (T < 0 || out_width < 1 || in_width < 1) return 0;
-  const Plan p = plan_of(T, out_width, in_width);
+  const Plan p = plan_of(T, out_width, in_width, shared_wo(out_width, in_width));
   return p.chunks * (static_cast<int64_t>(out_width) * in_width + p.db_ld);
 }
 

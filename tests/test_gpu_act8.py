@@ -138,7 +138,9 @@ def _check_wgrad(dy, k, val, bias=True):
     (1, 128, 128, "f32", False), (0, 128, 64, "f32", False), (181, 128, 128, "f32", False), (181, 128, 512, "f32", True),
     (1037, 512, 128, "f32", False), (65, 65, 128, "f32", False), (300, 1, 32, "f32", True), (77, 33, 160, "f32", False),
     (130, 64, 96, "bf16", False), (257, 1000, 1024, "bf16", True), (500, 17, 32, "bf16", False), (15, 200, 288, "bf16", True),
-    (16, 64, 128, "f32", True), (17, 66, 64, "f32", False), (4100, 130, 256, "f32", False), (33, 7, 2048, "f32", False)])
+    (16, 64, 128, "f32", True), (17, 66, 64, "f32", False), (4100, 130, 256, "f32", False), (33, 7, 2048, "f32", False),
+    (70, 201, 160, "f32", False), (95, 333, 288, "bf16", True), (64, 127, 192, "bf16", False), (31, 128, 160, "f32", True),
+    (33, 600, 1312, "f32", False), (3000, 128, 256, "bf16", False)])
 def test_wgrad(gpu, T, out, W, dtype, relu):
     rng = np.random.default_rng(T + 3 * out + W)
     k = act8.pack(_x(rng, T, W, "f32", relu).to(gpu), relu=relu)
@@ -161,7 +163,8 @@ def test_wgrad_keeps_all_of_fp32(gpu):
 
 @pytest.mark.parametrize("T,out,W,dtype,relu", [
     (1, 128, 128, "f32", False), (0, 64, 64, "f32", False), (181, 512, 128, "f32", False), (1037, 512, 128, "f32", False),
-    (77, 96, 160, "f32", True), (130, 64, 96, "bf16", False), (257, 992, 544, "bf16", True), (9, 32, 32, "f32", False)])
+    (77, 96, 160, "f32", True), (130, 64, 96, "bf16", False), (257, 992, 544, "bf16", True), (9, 32, 32, "f32", False),
+    (130, 256, 288, "f32", False), (77, 128, 160, "bf16", True), (2049, 160, 1024, "f32", False)])
 def test_relu_wgrad(gpu, T, out, W, dtype, relu):
     rng = np.random.default_rng(T + 5 * out + W)
     x = act8.pack(_x(rng, T, W, "f32", relu).to(gpu), relu=relu)
