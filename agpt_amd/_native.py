@@ -111,6 +111,9 @@ EMBED_SYMBOLS = {
     "agpt_embed_bwd_workspace_floats": (C.c_int64, [C.c_int64, C.c_int]),
     "agpt_embed_bwd": (C.c_int, [_vp, C.c_int64, _vp, C.c_float, _vp, _vp, C.c_int64, C.c_int64, C.c_int64, C.c_int,
                                  C.c_int, _vp]),
+    "agpt_embed_bwd_tokens_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int64, C.c_int]),
+    "agpt_embed_bwd_tokens": (C.c_int, [_vp, C.c_int64, _vp, C.c_int, C.c_float, _vp, _vp, C.c_int64, C.c_int64, C.c_int64,
+                                        C.c_int, C.c_int, _vp]),
 }
 
 # include/agpt_act8.h (same library as the attention entry points).

@@ -4,7 +4,7 @@
 // added to by two workgroups.
 //
 // Sort: a stable counting sort of (token, row) by digits of up to 8 bits, low
-// digit first: per tile of 4096 rows a digit histogram, per digit a scan over
+// digit first: per tile of 2048 rows a digit histogram, per digit a scan over
 // the tiles, then each tile places its rows by ballots (equal digits of a wave
 // keep their lane order, waves their order through per-wave counts).
 //
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(kThreads) void embed_fwd_kernel(const T* __restrict
 }
 
 // ---- sort ----------------------------------------------------------------------
-constexpr int kTile = 4096;      // rows of a sort tile, kTile / kWaves of them per wave
+constexpr int kTile = 2048;      // rows of a sort tile, kTile / kWaves of them per wave
 constexpr int kMaxBits = 8;      // digit width
 constexpr int kDigits = 1 << kMaxBits;
 
@@ -115,14 +115,15 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(int32_t* __restrict__ co
 }
 
 // Places a tile's rows: digit start + rows of the digit in earlier tiles +
-// rank within the tile. kFirst: keys from the tokens, rows are 0, 1, ....
+// rank within the tile. kFirst: keys from the tokens, rows are 0, 1, .... offsets: where this is the only pass.
 template <typename I, bool kFirst>
 __global__ __launch_bounds__(kThreads) void place_kernel(const I* __restrict__ keys, const int32_t* __restrict__ rows,
                                                          int64_t n, int64_t vocab, int shift, int bits,
                                                          const int32_t* __restrict__ counts,
                                                          const int32_t* __restrict__ totals, int tiles,
                                                          int32_t* __restrict__ keys_out,
-                                                         int32_t* __restrict__ rows_out) {
+                                                         int32_t* __restrict__ rows_out,
+                                                         int32_t* __restrict__ offsets) {
   __shared__ int next[kWaves][kDigits];  // where the wave's next row of a digit goes
   __shared__ int wsum[kWaves];
   const int tid = thread_x(), lane = tid & 63, wave = tid >> 6, tile = block_x(), digits = 1 << bits;
@@ -141,6 +142,8 @@ __global__ __launch_bounds__(kThreads) void place_kernel(const I* __restrict__ k
   {
     const int tot = tid < digits ? totals[tid] : 0;
     int at = block_scan(tot, wsum) - tot;
+    // a single digit is the whole key: its starts are the plan's offsets
+    if (offsets != nullptr && tile == 0 && tid <= vocab) offsets[tid] = at;
     if (tid < digits) {
       at += counts[static_cast<int64_t>(tid) * tiles + tile];
       for (int w = 0; w < kWaves; ++w) {
@@ -263,23 +266,175 @@ __global__ __launch_bounds__(kThreads) void sums_kernel(const T* __restrict__ dx
 }
 
 // Workgroup `span`: the long token that begins in it and goes on past it, if
-// there is one: its pieces added in span order.
-__global__ __launch_bounds__(kThreads) void join_kernel(const float* __restrict__ part,
-                                                        const int32_t* __restrict__ keys,
-                                                        const int32_t* __restrict__ offsets, float scale,
-                                                        float* __restrict__ dE, int32_t n, int32_t vocab, int D, int R) {
-  const int span = block_x();
+// there is one: its pieces, dealt to slots of `lanes` columns, the slots added in order.
+constexpr int kJoin = 1024;
+__global__ __launch_bounds__(kJoin) void join_kernel(const float* __restrict__ part, const int32_t* __restrict__ keys,
+                                                     const int32_t* __restrict__ offsets, float scale,
+                                                     float* __restrict__ dE, int32_t n, int32_t vocab, int D, int R,
+                                                     int lanes) {
+  __shared__ float red[kJoin];
+  const int span = block_x(), tid = thread_x();
   const int32_t s0 = span * R, s1 = s0 + R < n ? s0 + R : n;
   const int32_t v = keys[s1 - 1];
   if (v >= vocab) return;
   const int32_t a = offsets[v], b = offsets[v + 1];
   if (b - a <= R || a < s0) return;
-  const int end = (b - 1) / R;
-  for (int c = thread_x(); c < D; c += kThreads) {
-    float s = part[(2 * static_cast<int64_t>(span) + 1) * D + c];
+  const int end = (b - 1) / R, slots = kJoin / lanes, slot = tid / lanes;
+  for (int c0 = 0; c0 < D; c0 += lanes) {
+    const int c = c0 + (tid & (lanes - 1));
+    float s = 0.0f;
+    if (c < D) {
+      if (slot == 0) s = part[(2 * static_cast<int64_t>(span) + 1) * D + c];
 #pragma unroll 8
-    for (int q = span + 1; q <= end; ++q) s += part[2 * static_cast<int64_t>(q) * D + c];
-    dE[static_cast<int64_t>(v) * D + c] = s * scale;
+      for (int q = span + 1 + slot; q <= end; q += slots) s += part[2 * static_cast<int64_t>(q) * D + c];
+    }
+    red[tid] = s;
+    __syncthreads();
+    if (slot == 0 && c < D) {
+      for (int q = 1; q < slots; ++q) s += red[q * lanes + tid];
+      dE[static_cast<int64_t>(v) * D + c] = s * scale;
+    }
+    __syncthreads();
+  }
+}
+
+// ---- one launch for short batches --------------------------------------------------
+// A workgroup owns the tokens v = range (mod ranges), ranges a power of two (so
+// that neighbouring, often equally frequent ids part), and 64 V columns. It reads
+// every token of the batch from L2, lists the rows of its own, sorts the list
+// (stable, by the token's number within the range: at most 256, one digit) and
+// sums each token's rows, a wave per token; a token of many rows takes all waves.
+constexpr int kDirect = 512, kDirectWaves = kDirect / 64;
+constexpr int kLocal = 256;  // tokens of a range at most
+
+template <typename T, typename I, int V, int kCap>
+__global__ __launch_bounds__(kDirect) void direct_kernel(const T* __restrict__ dx, int64_t ld,
+                                                         const I* __restrict__ tokens, float scale,
+                                                         float* __restrict__ dE, int n, int64_t vocab, int D, int log_ranges,
+                                                         int lanes) {
+  __shared__ uint16_t found[kCap + kDirect], rows[kCap + kDirect];
+  __shared__ int next[kDirectWaves][kLocal];
+  __shared__ int start[kLocal + 1];
+  __shared__ int wsum[kDirectWaves];
+  __shared__ float red[kDirect * V];
+  const int tid = thread_x(), lane = tid & 63, wave = tid >> 6, blk = block_x();
+  const int ranges = 1 << log_ranges, range = blk & (ranges - 1), slice = blk >> log_ranges;
+  const int per_range = static_cast<int>((vocab + ranges - 1) >> log_ranges);
+  const uint64_t below = (1ull << lane) - 1;
+
+  const int share = (n + kDirect - 1) / kDirect * 64, first = wave * share;
+  const int last = first + share < n ? first + share : n;
+  int cnt = 0;
+  for (int i = first; i < last; i += 4 * 64) {
+    I tok[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) tok[u] = i + u * 64 + lane < last ? tokens[i + u * 64 + lane] : static_cast<I>(-1);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t t = static_cast<int64_t>(tok[u]);
+      const bool mine = t >= 0 && t < vocab && (static_cast<int>(t) & (ranges - 1)) == range;
+      const uint64_t m = __ballot(mine);
+      if (mine) found[first + cnt + __popcll(m & below)] = static_cast<uint16_t>(i + u * 64 + lane);
+      cnt += __popcll(m);
+    }
+  }
+  for (int i = lane; i < kLocal; i += 64) next[wave][i] = 0;
+  __builtin_amdgcn_wave_barrier();
+  auto local_of = [&](int row) { return static_cast<int>(static_cast<int64_t>(tokens[row]) >> log_ranges); };
+  for (int j = lane; j < cnt; j += 64) atomicAdd(&next[wave][local_of(found[first + j])], 1);
+  __syncthreads();
+  {
+    int tot = 0;
+    if (tid < kLocal)
+      for (int w = 0; w < kDirectWaves; ++w) tot += next[w][tid];
+    int inc = tot;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const int u = __shfl_up(inc, o);
+      if (lane >= o) inc += u;
+    }
+    if (lane == 63) wsum[wave] = inc;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) inc += wsum[w];
+    if (tid < kLocal) {
+      int at = inc - tot;
+      start[tid] = at;
+      if (tid == kLocal - 1) start[kLocal] = inc;
+      for (int w = 0; w < kDirectWaves; ++w) {
+        const int c = next[w][tid];
+        next[w][tid] = at;
+        at += c;
+      }
+    }
+  }
+  __syncthreads();
+  for (int j = 0; j < cnt; j += 64) {
+    const bool in = j + lane < cnt;
+    const int row = in ? found[first + j + lane] : 0;
+    const int d = in ? local_of(row) : 0;
+    uint64_t same = __ballot(in);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const uint64_t set = __ballot((d >> b) & 1);
+      same &= ((d >> b) & 1) ? set : ~set;
+    }
+    const int rank = __popcll(same & below);
+    int at = 0;
+    if (in) at = next[wave][d] + rank;
+    __builtin_amdgcn_wave_barrier();
+    if (in && rank == 0) next[wave][d] = at + __popcll(same);
+    __builtin_amdgcn_wave_barrier();
+    if (in) rows[at] = static_cast<uint16_t>(row);
+  }
+  __syncthreads();
+
+  const int groups = 64 / lanes, grp = lane / lanes, c = slice * 64 * V + (lane & (lanes - 1)) * V;
+  const int kLong = 64 * groups;  // rows that a wave sums by itself
+  auto sum_rows = [&](int a, int b, float (&s)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] = 0.0f;
+    if (c < D) {
+#pragma unroll 8
+      for (int j = a + grp; j < b; j += groups) {
+        float x[V];
+        load_row<V>(dx + rows[j] * ld + c, x);
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] += x[i];
+      }
+    }
+    for (int o = lanes; o < 64; o *= 2)
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] += __shfl_xor(s[i], o);
+  };
+  for (int k = wave; k < per_range; k += kDirectWaves) {
+    const int64_t v = (static_cast<int64_t>(k) << log_ranges) | range;
+    const int a = start[k], b = start[k + 1];
+    if (v >= vocab || b - a > kLong) continue;
+    float s[V];
+    sum_rows(a, b, s);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] *= scale;
+    if (grp == 0 && c < D) store_row<V>(dE + v * D + c, s);
+  }
+  for (int k = 0; k < per_range; ++k) {
+    const int a = start[k], b = start[k + 1];
+    if (b - a <= kLong) continue;
+    const int64_t v = (static_cast<int64_t>(k) << log_ranges) | range;
+    const int each = (b - a + kDirectWaves - 1) / kDirectWaves, w0 = a + wave * each;
+    float s[V];
+    sum_rows(w0 < b ? w0 : b, w0 + each < b ? w0 + each : b, s);
+#pragma unroll
+    for (int i = 0; i < V; ++i) red[tid * V + i] = s[i];
+    __syncthreads();
+    if (wave == 0 && grp == 0 && c < D) {
+      for (int w = 1; w < kDirectWaves; ++w)
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] += red[(w * 64 + lane) * V + i];
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] *= scale;
+      store_row<V>(dE + v * D + c, s);
+    }
+    __syncthreads();
   }
 }
 
@@ -316,6 +471,11 @@ int check_counts(const char* what, int64_t T, int64_t V) {
   if (T < 0 || V < 1) return invalid(what, "T < 0 or V < 1");
   if (T > kMaxCount || V > kMaxCount) return invalid(what, "T and V must be below 2^31 - 4096");
   return AGPT_OK;
+}
+
+// Whether rows of dx and of the table go in 16-byte pieces.
+bool wide_rows(int D, int64_t ld, int es, const void* dx, const void* table) {
+  return static_cast<int64_t>(D) * es % 16 == 0 && ld * es % 16 == 0 && aligned(dx, 16) && aligned(table, 16);
 }
 
 template <typename Fn>
@@ -381,14 +541,14 @@ extern "C" int agpt_embed_plan(const void* tokens, int token_bits, int64_t T, in
     return invalid(what, "workspace smaller than agpt_embed_plan_workspace_bytes");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   int32_t *order = plan, *keys = plan + T, *offsets = plan + 2 * T;
+  int passes;
+  const int bits = digit_bits(V, &passes), digits = 1 << bits;
   if (T > 0) {
     const int tiles = static_cast<int>(tiles_of(T));
     int32_t* counts = static_cast<int32_t*>(workspace);
     int32_t* totals = counts + static_cast<int64_t>(kDigits) * tiles;
     int32_t* keys2 = totals + kDigits;
     int32_t* rows2 = keys2 + T;
-    int passes;
-    const int bits = digit_bits(V, &passes), digits = 1 << bits;
     const void* kin = tokens;
     const int32_t* rin = nullptr;
     for (int p = 0; p < passes; ++p) {
@@ -402,7 +562,7 @@ extern "C" int agpt_embed_plan(const void* tokens, int token_bits, int64_t T, in
                            tiles);
         hipLaunchKernelGGL(scan_kernel, dim3(digits), dim3(kThreads), 0, st, counts, tiles, totals);
         hipLaunchKernelGGL((place_kernel<I, kFirst>), dim3(tiles), dim3(kThreads), 0, st, k, rin, T, V, p * bits, bits,
-                           counts, totals, tiles, kout, rout);
+                           counts, totals, tiles, kout, rout, passes == 1 ? offsets : static_cast<int32_t*>(nullptr));
       };
       if (p > 0) go(int32_t{}, std::false_type{});
       else if (token_bits == 32) go(int32_t{}, std::true_type{});
@@ -411,7 +571,8 @@ extern "C" int agpt_embed_plan(const void* tokens, int token_bits, int64_t T, in
       rin = rout;
     }
   }
-  hipLaunchKernelGGL(offsets_kernel, dim3(static_cast<unsigned>(V / kThreads + 1)), dim3(kThreads), 0, st, keys,
+  if (T == 0 || passes > 1)
+    hipLaunchKernelGGL(offsets_kernel, dim3(static_cast<unsigned>(V / kThreads + 1)), dim3(kThreads), 0, st, keys,
                      static_cast<int32_t>(T), static_cast<int32_t>(V), offsets);
   return launch_status(what);
 }
@@ -447,7 +608,7 @@ extern "C" int agpt_embed_bwd(const void* dx, int64_t ld_dx, const int32_t* plan
   const int64_t waves = (V + kWaves - 1) / kWaves;
   if (waves + spans > 0x7fffffff) return invalid(what, "T and V too large together");
   const int32_t *order = plan, *keys = plan + T, *offsets = plan + 2 * T;
-  const bool wide = static_cast<int64_t>(D) * es % 16 == 0 && ld_dx * es % 16 == 0 && aligned(dx, 16) && aligned(d_table, 16);
+  const bool wide = wide_rows(D, ld_dx, es, dx, d_table);
   with_dtype(dtype, wide, [&](auto e, auto vc) {
     using E = decltype(e);
     constexpr int W = decltype(vc)::value;
@@ -456,7 +617,78 @@ extern "C" int agpt_embed_bwd(const void* dx, int64_t ld_dx, const int32_t* plan
                        static_cast<int32_t>(T), static_cast<int32_t>(V), D, R, spans, lanes_for(D, W));
   });
   if (const int rc = launch_status(what)) return rc;
-  hipLaunchKernelGGL(join_kernel, dim3(spans), dim3(kThreads), 0, st, workspace, keys, offsets, scale, d_table,
-                     static_cast<int32_t>(T), static_cast<int32_t>(V), D, R);
+  int lanes = 1;
+  while (lanes < D && lanes < 128) lanes *= 2;
+  hipLaunchKernelGGL(join_kernel, dim3(spans), dim3(kJoin), 0, st, workspace, keys, offsets, scale, d_table,
+                     static_cast<int32_t>(T), static_cast<int32_t>(V), D, R, lanes);
+  return launch_status(what);
+}
+
+namespace {
+
+// The one-launch form: log2 of its ranges, or -1 where sorting first is taken.
+// Every workgroup reads all tokens, so it is for batches of at most kDirectRows
+// rows, and for at most kDirectReads token reads in all.
+constexpr int64_t kDirectRows = 16384, kDirectReads = int64_t{1} << 25;
+int direct_ranges(int64_t T, int64_t V, int D, int width) {
+  if (T < 1 || T > kDirectRows) return -1;
+  const int64_t slices = (D + 64 * width - 1) / (64 * width);
+  int lr = 0;
+  while ((static_cast<int64_t>(kLocal) << lr) < V || ((slices << lr) < 512 && (int64_t{1} << lr) < V)) ++lr;
+  return (slices << lr) * T <= kDirectReads ? lr : -1;
+}
+
+}  // namespace
+
+// The plan, then the larger of what making it and summing by it need.
+extern "C" int64_t agpt_embed_bwd_tokens_workspace_bytes(int64_t T, int64_t V, int D) {
+  if (T < 0 || V < 1 || D < 1) return 0;
+  const int64_t a = agpt_embed_plan_workspace_bytes(T, V), b = 4 * agpt_embed_bwd_workspace_floats(T, D);
+  return 4 * agpt_embed_plan_ints(T, V) + (a > b ? a : b);
+}
+
+extern "C" int agpt_embed_bwd_tokens(const void* dx, int64_t ld_dx, const void* tokens, int token_bits, float scale,
+                                     float* d_table, void* workspace, int64_t workspace_bytes, int64_t T, int64_t V, int D,
+                                     int dtype, void* stream) {
+  const char* what = "agpt_embed_bwd_tokens";
+  if (const int rc = check_counts(what, T, V)) return rc;
+  if (D < 1 || ld_dx < D) return invalid(what, "D < 1 or a row stride smaller than D");
+  if (token_bits != 32 && token_bits != 64) return invalid(what, "token_bits must be 32 or 64");
+  if (dtype != AGPT_DTYPE_F32 && dtype != AGPT_DTYPE_BF16) return invalid(what, "unknown dtype");
+  if (!d_table || !workspace || (T > 0 && (!dx || !tokens))) return invalid(what, "null pointer");
+  const int es = dtype == AGPT_DTYPE_F32 ? 4 : 2;
+  if (!aligned(dx, es) || !aligned(tokens, token_bits / 8) || !aligned(d_table, 4) || !aligned(workspace, 4))
+    return invalid(what, "a pointer is not aligned to its elements");
+  if (workspace_bytes < agpt_embed_bwd_tokens_workspace_bytes(T, V, D))
+    return invalid(what, "workspace smaller than agpt_embed_bwd_tokens_workspace_bytes");
+  const bool wide = wide_rows(D, ld_dx, es, dx, d_table);
+  const int width = !wide ? 1 : (dtype == AGPT_DTYPE_F32 ? 4 : 8);
+  const int lr = direct_ranges(T, V, D, width);
+  if (lr < 0) {
+    int32_t* plan = static_cast<int32_t*>(workspace);
+    int32_t* rest = plan + agpt_embed_plan_ints(T, V);
+    const int64_t bytes = workspace_bytes - 4 * agpt_embed_plan_ints(T, V);
+    if (const int rc = agpt_embed_plan(tokens, token_bits, T, V, plan, rest, bytes, stream)) return rc;
+    return agpt_embed_bwd(dx, ld_dx, plan, scale, d_table, reinterpret_cast<float*>(rest), bytes / 4, T, V, D, dtype, stream);
+  }
+  with_dtype(dtype, wide, [&](auto e, auto vc) {
+    using E = decltype(e);
+    constexpr int W = decltype(vc)::value;
+    int lanes = 1;
+    while (lanes * W < D && lanes < 64) lanes *= 2;
+    const dim3 grid(static_cast<unsigned>(((D + 64 * W - 1) / (64 * W)) << lr));
+    auto go = [&](auto tok, auto cap) {
+      using I = decltype(tok);
+      hipLaunchKernelGGL((direct_kernel<E, I, W, decltype(cap)::value>), grid, dim3(kDirect), 0,
+                         static_cast<hipStream_t>(stream), static_cast<const E*>(dx), ld_dx, static_cast<const I*>(tokens),
+                         scale, d_table, static_cast<int>(T), V, D, lr, lanes);
+    };
+    auto size = [&](auto tok) {
+      if (T <= 2048) go(tok, std::integral_constant<int, 2048>{});
+      else go(tok, std::integral_constant<int, kDirectRows>{});
+    };
+    if (token_bits == 32) size(int32_t{});
+    else size(int64_t{});
+  });
   return launch_status(what);
 }

@@ -66,27 +66,36 @@ def embed_bwd(dx, tokens, vocab: int | None = None, scale: float = 1.0, out=None
     """d_table [V, D] fp32 = scale * the sum of dx's rows by token. tokens: the
     batch's tokens (sorted in this call; vocab needed) or its EmbedPlan. dx
     [T, D] fp32 or bf16; rows may be strided."""
-    if not isinstance(tokens, EmbedPlan):
-        if vocab is None:
-            raise ValueError("vocab is needed with tokens that are not planned")
-        tokens = EmbedPlan(tokens, vocab)
-    elif vocab is not None and vocab != tokens.vocab:
-        raise ValueError("the plan has another vocabulary")
-    plan = tokens
-    _check_cuda("dx", dx, plan.device)
+    plan = tokens if isinstance(tokens, EmbedPlan) else None
+    if plan is None:
+        bits = _tokens(tokens)
+        if vocab is None or vocab < 1:
+            raise ValueError("vocab, at least 1, is needed with tokens that are not planned")
+        n_rows, device = tokens.shape[0], tokens.device
+    else:
+        if vocab is not None and vocab != plan.vocab:
+            raise ValueError("the plan has another vocabulary")
+        vocab, n_rows, device = plan.vocab, plan.T, plan.device
+    _check_cuda("dx", dx, device)
     dt, ld = _dtype("dx", dx), _rows("dx", dx)
     T, D = dx.shape
-    if T != plan.T or D < 1:
+    if T != n_rows or D < 1:
         raise ValueError("dx must have one row per token, at least one wide")
     if out is None:
-        out = torch.empty(plan.vocab, D, device=dx.device, dtype=torch.float32)
+        out = torch.empty(vocab, D, device=device, dtype=torch.float32)
     else:
-        _check_cuda("out", out, dx.device)
-        if out.shape != (plan.vocab, D) or out.dtype != torch.float32 or not out.is_contiguous():
+        _check_cuda("out", out, device)
+        if out.shape != (vocab, D) or out.dtype != torch.float32 or not out.is_contiguous():
             raise ValueError("out must be a contiguous float32 [vocab, D] tensor")
     lib = _native.attn_lib()
+    if plan is None:
+        n = lib.agpt_embed_bwd_tokens_workspace_bytes(T, vocab, D)
+        ws = torch.empty(n, device=device, dtype=torch.uint8)
+        _launch(device, lambda: lib.agpt_embed_bwd_tokens(
+            _ptr(dx), ld, _ptr(tokens), bits, C.c_float(scale), _ptr(out), _ptr(ws), n, T, vocab, D, dt, _stream(dx)))
+        return out
     n = lib.agpt_embed_bwd_workspace_floats(T, D)
-    ws = torch.empty(n, device=dx.device, dtype=torch.float32)
-    _launch(dx.device, lambda: lib.agpt_embed_bwd(
-        _ptr(dx), ld, _ptr(plan.rows), C.c_float(scale), _ptr(out), _ptr(ws), n, T, plan.vocab, D, dt, _stream(dx)))
+    ws = torch.empty(n, device=device, dtype=torch.float32)
+    _launch(device, lambda: lib.agpt_embed_bwd(
+        _ptr(dx), ld, _ptr(plan.rows), C.c_float(scale), _ptr(out), _ptr(ws), n, T, vocab, D, dt, _stream(dx)))
     return out

@@ -51,6 +51,15 @@ int64_t agpt_embed_bwd_workspace_floats(int64_t T, int D);
 int agpt_embed_bwd(const void* dx, int64_t ld_dx, const int32_t* plan, float scale, float* d_table, float* workspace,
                    int64_t workspace_floats, int64_t T, int64_t V, int D, int dtype, void* stream);
 
+/* The same from the tokens themselves, for a batch that comes once: short
+ * batches in one launch that sorts each token range on the fly, longer ones by a
+ * plan made in the workspace (at least agpt_embed_bwd_tokens_workspace_bytes
+ * bytes). Its sums may be in another order than a plan's; the order depends on
+ * the tokens and sizes alone. */
+int64_t agpt_embed_bwd_tokens_workspace_bytes(int64_t T, int64_t V, int D);
+int agpt_embed_bwd_tokens(const void* dx, int64_t ld_dx, const void* tokens, int token_bits, float scale, float* d_table,
+                          void* workspace, int64_t workspace_bytes, int64_t T, int64_t V, int D, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

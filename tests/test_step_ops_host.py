@@ -64,6 +64,18 @@ def test_embed_bwd_refuses(kw, part):
                                                a["V"], a["D"], a["dtype"], None), BAD, part)
 
 
+@pytest.mark.parametrize("kw,part", [
+    (dict(T=-1), "T < 0"), (dict(V=0), "V < 1"), (dict(V=2**31 - 1), "2^31"), (dict(D=0), "D < 1"),
+    (dict(ld=7), "row stride"), (dict(bits=8), "token_bits"), (dict(dtype=2), "dtype"), (dict(dx=None), "null"),
+    (dict(tokens=None), "null"), (dict(dE=None), "null"), (dict(ws=None), "null"), (dict(n=3), "workspace"),
+    (dict(dx=P + 2), "aligned"), (dict(tokens=P + 2), "aligned")])
+def test_embed_bwd_tokens_refuses(kw, part):
+    a = dict(dx=P, ld=8, tokens=P, bits=32, dE=P, ws=P, n=1 << 30, T=300, V=5, D=8, dtype=0)
+    a.update(kw)
+    _refuses(_native.attn_lib().agpt_embed_bwd_tokens(a["dx"], a["ld"], a["tokens"], a["bits"], C.c_float(1), a["dE"],
+                                                      a["ws"], a["n"], a["T"], a["V"], a["D"], a["dtype"], None), BAD, part)
+
+
 QK = dict(qkv=P, ld=192, bias=P, wq=P, wk=P, pos=P, cos=P, sin=P, seq=32, T=3, H=2, Hk=1, hd=48, dtype=0, q=P, k=P, v=P)
 
 
