@@ -8,10 +8,9 @@
 // the tiles, then each tile places its rows by ballots (equal digits of a wave
 // keep their lane order, waves their order through per-wave counts).
 //
-// Sums: the sorted rows are cut into spans of R. A token of up to R rows is
-// summed by one wave that gathers its rows; a longer one is summed piecewise,
-// at most two pieces per span (the end of one long token and the start of the
-// next), and its pieces are added in span order.
+// Sums: a token of up to 16 rows is summed by one group of lanes that gathers
+// them; a longer one by workgroups over spans of the sorted rows, and the pieces
+// of one that goes over several spans are added in span order.
 
 #include "rows.h"
 #include "../../include/agpt_embed.h"
@@ -24,6 +23,7 @@ using namespace agpt_rows;
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
+constexpr int kMaxSpan = 512;
 
 // ---- lookup ------------------------------------------------------------------
 // `lanes` threads (a power of two) hold a row in pieces of V elements; a
@@ -193,23 +193,16 @@ __global__ __launch_bounds__(kThreads) void offsets_kernel(const int32_t* __rest
 }
 
 // ---- sums ----------------------------------------------------------------------
-// Workgroups 0 .. spans - 1: the pieces of long tokens in their span, to
-// part[2 span] (a token begun in an earlier span) and part[2 span + 1] (one
-// that begins here and goes on past the span). The others: a wave per token
-// of up to R rows, zeros where it has none.
-template <typename T, int V>
-__device__ __forceinline__ void gather_sum(const T* __restrict__ dx, int64_t ld, const int32_t* __restrict__ order,
-                                           int a, int b, int step, int c, float (&s)[V]) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) s[i] = 0.0f;
-#pragma unroll 8
-  for (int j = a; j < b; j += step) {
-    float v[V];
-    load_row<V>(dx + order[j] * ld + c, v);
-#pragma unroll
-    for (int i = 0; i < V; ++i) s[i] += v[i];
-  }
-}
+// Workgroups 0 .. spans - 1 take a span of sorted rows each. A token of up to
+// kShort rows is summed by a group of lanes in the span where it begins. A longer
+// one is summed by the whole workgroup, at once where it lies in one span, else in
+// pieces to part[2 span] (begun in an earlier span) and part[2 span + 1] (begins
+// here). The workgroups after them write the zeros of the tokens without rows:
+// written among the gathers, they fill the memory's queues in front of its reads
+// (16K rows over 50,000 tokens of 1024 bf16 from HBM: 84 us together, XX in this order).
+constexpr int kShort = 16;
+constexpr int kTokens = 4;   // of a lane group at a time, their first rows on their way together
+constexpr int kZeroRows = 64;
 
 template <typename T, int V>
 __global__ __launch_bounds__(kThreads) void sums_kernel(const T* __restrict__ dx, int64_t ld,
@@ -218,24 +211,52 @@ __global__ __launch_bounds__(kThreads) void sums_kernel(const T* __restrict__ dx
                                                         const int32_t* __restrict__ offsets, float scale,
                                                         float* __restrict__ dE, float* __restrict__ part, int32_t n,
                                                         int32_t vocab, int D, int R, int spans, int lanes) {
-  __shared__ float red[kThreads * V];
   const int tid = thread_x(), blk = block_x();
   if (blk < spans) {
+    __shared__ float red[kThreads * V];
+    __shared__ int32_t many[kMaxSpan / kShort + 1], few_at[kMaxSpan], few_v[kMaxSpan], few_n[kMaxSpan];
+    __shared__ int n_many, n_few;
     const int32_t s0 = blk * R, s1 = s0 + R < n ? s0 + R : n;
-    const int32_t first = keys[s0], last = keys[s1 - 1];
-    for (int piece = 0; piece < 2; ++piece) {
-      const int32_t v = piece ? last : first;
+    if (tid == 0) n_many = n_few = 0;
+    __syncthreads();
+    // the span's tokens (listed in any order, each has a sum of its own): the short ones that begin in it, the
+    // long ones that do and the one that it begins within
+    for (int32_t p = s0 + tid; p < s1; p += kThreads) {
+      const int32_t v = keys[p];
       if (v >= vocab) continue;
-      const int32_t a = offsets[v], b = offsets[v + 1];
-      if (b - a <= R || (a < s0) != (piece == 0)) continue;
+      const int32_t a = offsets[v];
+      if (a != p && p != s0) continue;
+      const int32_t count = offsets[v + 1] - a;
+      if (count > kShort) {
+        many[atomicAdd(&n_many, 1)] = v;
+      } else if (a == p) {
+        const int q = atomicAdd(&n_few, 1);
+        few_at[q] = p;
+        few_v[q] = v;
+        few_n[q] = count;
+      }
+    }
+    __syncthreads();
+    const int slots = kThreads / lanes, slot = tid / lanes;
+    for (int m = 0; m < n_many; ++m) {
+      const int32_t v = many[m], a = offsets[v], b = offsets[v + 1];
       const int32_t p0 = a > s0 ? a : s0, p1 = b < s1 ? b : s1;
-      const int slots = kThreads / lanes, slot = tid / lanes;
+      const bool whole = a >= s0 && b <= s1;
+      float* out = whole ? dE + static_cast<int64_t>(v) * D : part + (2 * static_cast<int64_t>(blk) + (a >= s0)) * D;
       for (int c0 = 0; c0 < D; c0 += lanes * V) {
         const int c = c0 + (tid & (lanes - 1)) * V;
         float s[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) s[i] = 0.0f;
-        if (c < D) gather_sum<T, V>(dx, ld, order, p0 + slot, p1, slots, c, s);
+        if (c < D) {
+#pragma unroll 8
+          for (int j = p0 + slot; j < p1; j += slots) {
+            float x[V];
+            load_row<V>(dx + order[j] * ld + c, x);
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[i] += x[i];
+          }
+        }
 #pragma unroll
         for (int i = 0; i < V; ++i) red[tid * V + i] = s[i];
         __syncthreads();
@@ -243,131 +264,179 @@ __global__ __launch_bounds__(kThreads) void sums_kernel(const T* __restrict__ dx
           for (int q = 1; q < slots; ++q)
 #pragma unroll
             for (int i = 0; i < V; ++i) s[i] += red[(q * lanes + tid) * V + i];
-          float* out = part + (2 * static_cast<int64_t>(blk) + piece) * D + c;
 #pragma unroll
-          for (int i = 0; i < V; ++i) out[i] = s[i];
+          for (int i = 0; i < V; ++i) out[c + i] = whole ? s[i] * scale : s[i];
         }
         __syncthreads();
       }
     }
+    for (int q = slot * kTokens; q < n_few; q += slots * kTokens) {
+      int32_t at[kTokens], count[kTokens], row[kTokens];
+#pragma unroll
+      for (int k = 0; k < kTokens; ++k) {
+        const bool in = q + k < n_few;
+        at[k] = in ? few_at[q + k] : 0;
+        count[k] = in ? few_n[q + k] : 0;
+        row[k] = in ? order[at[k]] : 0;
+      }
+      for (int c = (tid & (lanes - 1)) * V; c < D; c += lanes * V) {
+        float s[kTokens][V];
+#pragma unroll
+        for (int k = 0; k < kTokens; ++k)
+          if (count[k] > 0) load_row<V>(dx + row[k] * ld + c, s[k]);
+#pragma unroll
+        for (int k = 0; k < kTokens; ++k) {
+          if (count[k] == 0) continue;
+#pragma unroll 8
+          for (int j = 1; j < count[k]; ++j) {
+            float x[V];
+            load_row<V>(dx + order[at[k] + j] * ld + c, x);
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[k][i] += x[i];
+          }
+#pragma unroll
+          for (int i = 0; i < V; ++i) s[k][i] *= scale;
+          store_row<V>(dE + static_cast<int64_t>(few_v[q + k]) * D + c, s[k]);
+        }
+      }
+    }
     return;
   }
-  const int64_t v = static_cast<int64_t>(blk - spans) * kWaves + (tid >> 6);
-  if (v >= vocab) return;
-  const int32_t a = offsets[v], b = offsets[v + 1];
-  if (b - a > R) return;
-  for (int c = (tid & 63) * V; c < D; c += 64 * V) {
-    float s[V];
-    gather_sum<T, V>(dx, ld, order, a, b, 1, c, s);
+  __shared__ int32_t off[kZeroRows + 1];
+  const int64_t v0 = static_cast<int64_t>(blk - spans) * kZeroRows;
+  if (tid <= kZeroRows) off[tid] = offsets[v0 + tid < vocab ? v0 + tid : vocab];
+  __syncthreads();
+  float zero[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[i] *= scale;
-    store_row<V>(dE + v * D + c, s);
+  for (int i = 0; i < V; ++i) zero[i] = 0.0f;
+  const int rows = kThreads / lanes;
+  for (int k = tid / lanes; k < kZeroRows && v0 + k < vocab; k += rows) {
+    if (off[k + 1] > off[k]) continue;
+    for (int c = (tid & (lanes - 1)) * V; c < D; c += lanes * V) store_row<V>(dE + (v0 + k) * D + c, zero);
   }
 }
 
-// Workgroup `span`: the long token that begins in it and goes on past it, if
-// there is one: its pieces, dealt to slots of `lanes` columns, the slots added in order.
+// The long tokens that begin in one of a workgroup's `each` spans and go on past
+// it: their pieces, dealt to slots of `lanes` columns, the slots added in order.
 constexpr int kJoin = 1024;
 __global__ __launch_bounds__(kJoin) void join_kernel(const float* __restrict__ part, const int32_t* __restrict__ keys,
                                                      const int32_t* __restrict__ offsets, float scale,
                                                      float* __restrict__ dE, int32_t n, int32_t vocab, int D, int R,
-                                                     int lanes) {
+                                                     int lanes, int spans, int each) {
   __shared__ float red[kJoin];
-  const int span = block_x(), tid = thread_x();
-  const int32_t s0 = span * R, s1 = s0 + R < n ? s0 + R : n;
-  const int32_t v = keys[s1 - 1];
-  if (v >= vocab) return;
-  const int32_t a = offsets[v], b = offsets[v + 1];
-  if (b - a <= R || a < s0) return;
-  const int end = (b - 1) / R, slots = kJoin / lanes, slot = tid / lanes;
-  for (int c0 = 0; c0 < D; c0 += lanes) {
-    const int c = c0 + (tid & (lanes - 1));
-    float s = 0.0f;
-    if (c < D) {
-      if (slot == 0) s = part[(2 * static_cast<int64_t>(span) + 1) * D + c];
+  __shared__ int32_t many[kJoin];
+  __shared__ int n_many;
+  const int tid = thread_x(), slots = kJoin / lanes, slot = tid / lanes;
+  const int c = block_y() * lanes + (tid & (lanes - 1));
+  for (int first = block_x() * each, last = first + each; first < last; first += kJoin) {
+    if (tid == 0) n_many = 0;
+    __syncthreads();
+    const int span = first + tid;
+    if (span < last && span < spans) {
+      const int32_t s0 = span * R, s1 = s0 + R < n ? s0 + R : n, v = keys[s1 - 1];
+      if (v < vocab) {
+        const int32_t a = offsets[v], b = offsets[v + 1];
+        if (b - a > kShort && a >= s0 && b > s1) many[atomicAdd(&n_many, 1)] = span;  // (in any order)
+      }
+    }
+    __syncthreads();
+    const int found = n_many;
+    for (int m = 0; m < found; ++m) {
+      const int s0 = many[m];
+      const int32_t v = keys[s0 * R + R - 1], end = (offsets[v + 1] - 1) / R;
+      float s = 0.0f;
+      if (c < D) {
+        if (slot == 0) s = part[(2 * static_cast<int64_t>(s0) + 1) * D + c];
 #pragma unroll 8
-      for (int q = span + 1 + slot; q <= end; q += slots) s += part[2 * static_cast<int64_t>(q) * D + c];
+        for (int q = s0 + 1 + slot; q <= end; q += slots) s += part[2 * static_cast<int64_t>(q) * D + c];
+      }
+      red[tid] = s;
+      __syncthreads();
+      if (slot == 0 && c < D) {
+        for (int q = 1; q < slots; ++q) s += red[q * lanes + tid];
+        dE[static_cast<int64_t>(v) * D + c] = s * scale;
+      }
+      __syncthreads();
     }
-    red[tid] = s;
-    __syncthreads();
-    if (slot == 0 && c < D) {
-      for (int q = 1; q < slots; ++q) s += red[q * lanes + tid];
-      dE[static_cast<int64_t>(v) * D + c] = s * scale;
-    }
-    __syncthreads();
   }
 }
 
-// ---- one launch for short batches --------------------------------------------------
-// A workgroup owns the tokens v = range (mod ranges), ranges a power of two (so
-// that neighbouring, often equally frequent ids part), and 64 V columns. It reads
-// every token of the batch from L2, lists the rows of its own, sorts the list
-// (stable, by the token's number within the range: at most 256, one digit) and
-// sums each token's rows, a wave per token; a token of many rows takes all waves.
-constexpr int kDirect = 512, kDirectWaves = kDirect / 64;
-constexpr int kLocal = 256;  // tokens of a range at most
+__global__ __launch_bounds__(kThreads) void zero_kernel(float* __restrict__ p, int64_t n, int gx) {
+  for (int64_t i = static_cast<int64_t>(block_x()) * kThreads + thread_x(); i < n; i += static_cast<int64_t>(gx) * kThreads)
+    p[i] = 0.0f;
+}
 
-template <typename T, typename I, int V, int kCap>
-__global__ __launch_bounds__(kDirect) void direct_kernel(const T* __restrict__ dx, int64_t ld,
-                                                         const I* __restrict__ tokens, float scale,
-                                                         float* __restrict__ dE, int n, int64_t vocab, int D, int log_ranges,
-                                                         int lanes) {
-  __shared__ uint16_t found[kCap + kDirect], rows[kCap + kDirect];
-  __shared__ int next[kDirectWaves][kLocal];
-  __shared__ int start[kLocal + 1];
-  __shared__ int wsum[kDirectWaves];
-  __shared__ float red[kDirect * V];
-  const int tid = thread_x(), lane = tid & 63, wave = tid >> 6, blk = block_x();
-  const int ranges = 1 << log_ranges, range = blk & (ranges - 1), slice = blk >> log_ranges;
-  const int per_range = static_cast<int>((vocab + ranges - 1) >> log_ranges);
+// ---- plans of short batches in one launch -----------------------------------------
+constexpr int kList = 512, kListWaves = kList / 64;
+constexpr int kLocal = 256;  // tokens of a workgroup's share of the vocabulary, at most
+
+// Lists the rows (n of them) whose token `mine` takes, in row order, each wave
+// over its own part of the batch: found[first of the wave ...], the wave's count
+// returned; `each` sees every key. Keys are the tokens, V for padding.
+template <typename I, typename Mine, typename Each>
+__device__ __forceinline__ int list_rows(const I* __restrict__ tokens, int n, int64_t vocab, uint16_t* found, int first,
+                                         int last, Mine&& mine, Each&& each) {
+  const int lane = thread_x() & 63;
   const uint64_t below = (1ull << lane) - 1;
-
-  const int share = (n + kDirect - 1) / kDirect * 64, first = wave * share;
-  const int last = first + share < n ? first + share : n;
+  constexpr int kFlight = 16;  // token loads in flight
   int cnt = 0;
-  for (int i = first; i < last; i += 4 * 64) {
-    I tok[4];
+  for (int i = first; i < last; i += kFlight * 64) {
+    I tok[kFlight];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) tok[u] = i + u * 64 + lane < last ? tokens[i + u * 64 + lane] : static_cast<I>(-1);
+    for (int u = 0; u < kFlight; ++u) tok[u] = i + u * 64 + lane < last ? tokens[i + u * 64 + lane] : I{0};
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t t = static_cast<int64_t>(tok[u]);
-      const bool mine = t >= 0 && t < vocab && (static_cast<int>(t) & (ranges - 1)) == range;
-      const uint64_t m = __ballot(mine);
-      if (mine) found[first + cnt + __popcll(m & below)] = static_cast<uint16_t>(i + u * 64 + lane);
+    for (int u = 0; u < kFlight; ++u) {
+      const bool in = i + u * 64 + lane < last;
+      const int32_t k = key_of(tok[u], vocab);
+      each(in, k);
+      const bool take = in && mine(k);
+      const uint64_t m = __ballot(take);
+      if (take) found[first + cnt + __popcll(m & below)] = static_cast<uint16_t>(i + u * 64 + lane);
       cnt += __popcll(m);
     }
   }
-  for (int i = lane; i < kLocal; i += 64) next[wave][i] = 0;
-  __builtin_amdgcn_wave_barrier();
-  auto local_of = [&](int row) { return static_cast<int>(static_cast<int64_t>(tokens[row]) >> log_ranges); };
-  for (int j = lane; j < cnt; j += 64) atomicAdd(&next[wave][local_of(found[first + j])], 1);
+  return cnt;
+}
+
+// next[wave][local] from the counts of a wave's listed rows to the first place of
+// its rows of that local token; start[local] the token's first place (and
+// start[kLocal] the listed rows' number). `mark(local, rows)` per local token.
+template <typename Mark>
+__device__ __forceinline__ void list_places(int (*next)[kLocal], int* start, int* wsum, Mark&& mark) {
+  const int tid = thread_x(), lane = tid & 63, wave = tid >> 6;
   __syncthreads();
-  {
-    int tot = 0;
-    if (tid < kLocal)
-      for (int w = 0; w < kDirectWaves; ++w) tot += next[w][tid];
-    int inc = tot;
+  int tot = 0;
+  if (tid < kLocal)
+    for (int w = 0; w < kListWaves; ++w) tot += next[w][tid];
+  int inc = tot;
 #pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-      const int u = __shfl_up(inc, o);
-      if (lane >= o) inc += u;
-    }
-    if (lane == 63) wsum[wave] = inc;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) inc += wsum[w];
-    if (tid < kLocal) {
-      int at = inc - tot;
-      start[tid] = at;
-      if (tid == kLocal - 1) start[kLocal] = inc;
-      for (int w = 0; w < kDirectWaves; ++w) {
-        const int c = next[w][tid];
-        next[w][tid] = at;
-        at += c;
-      }
+  for (int o = 1; o < 64; o *= 2) {
+    const int u = __shfl_up(inc, o);
+    if (lane >= o) inc += u;
+  }
+  if (lane == 63) wsum[wave] = inc;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) inc += wsum[w];
+  if (tid < kLocal) {
+    int at = inc - tot;
+    start[tid] = at;
+    mark(tid, tot);
+    if (tid == kLocal - 1) start[kLocal] = inc;
+    for (int w = 0; w < kListWaves; ++w) {
+      const int c = next[w][tid];
+      next[w][tid] = at;
+      at += c;
     }
   }
   __syncthreads();
+}
+
+// The stable places of a wave's listed rows: place(row, local, at).
+template <typename Local, typename Place>
+__device__ __forceinline__ void list_sort(const uint16_t* found, int first, int cnt, int* next, Local&& local_of,
+                                          Place&& place) {
+  const int lane = thread_x() & 63;
+  const uint64_t below = (1ull << lane) - 1;
   for (int j = 0; j < cnt; j += 64) {
     const bool in = j + lane < cnt;
     const int row = in ? found[first + j + lane] : 0;
@@ -380,67 +449,137 @@ __global__ __launch_bounds__(kDirect) void direct_kernel(const T* __restrict__ d
     }
     const int rank = __popcll(same & below);
     int at = 0;
-    if (in) at = next[wave][d] + rank;
+    if (in) at = next[d] + rank;
     __builtin_amdgcn_wave_barrier();
-    if (in && rank == 0) next[wave][d] = at + __popcll(same);
+    if (in && rank == 0) next[d] = at + __popcll(same);
     __builtin_amdgcn_wave_barrier();
-    if (in) rows[at] = static_cast<uint16_t>(row);
+    if (in) place(row, d, at);
   }
+}
+
+// A workgroup owns the keys lo .. lo + per - 1 (of 0 .. V). It reads every token
+// from L2, counts those below lo, which is where its own begin, and lists and
+// sorts its own: no workgroup waits for another.
+constexpr int kShortRows = 16384;
+template <typename I>
+__global__ __launch_bounds__(kList) void short_plan_kernel(const I* __restrict__ tokens, int n, int64_t vocab, int per,
+                                                           int32_t* __restrict__ order, int32_t* __restrict__ keys,
+                                                           int32_t* __restrict__ offsets) {
+  __shared__ uint16_t found[kShortRows + kList];
+  __shared__ int next[kListWaves][kLocal];
+  __shared__ int start[kLocal + 1];
+  __shared__ int wsum[kListWaves], fewer[kListWaves];
+  const int tid = thread_x(), lane = tid & 63, wave = tid >> 6;
+  const int64_t lo = static_cast<int64_t>(block_x()) * per, hi = lo + per;
+  const int share = (n + kList - 1) / kList * 64, first = wave * share;
+  int under = 0;
+  const int cnt = list_rows(
+      tokens, n, vocab, found, first, first + share < n ? first + share : n,
+      [&](int32_t k) { return k >= lo && k < hi; },
+      [&](bool in, int32_t k) { under += __popcll(__ballot(in && k < lo)); });
+  for (int i = lane; i < kLocal; i += 64) next[wave][i] = 0;
+  if (lane == 0) fewer[wave] = under;
+  __builtin_amdgcn_wave_barrier();
+  auto local_of = [&](int row) { return static_cast<int>(key_of(tokens[row], vocab) - lo); };
+  for (int j = lane; j < cnt; j += 64) atomicAdd(&next[wave][local_of(found[first + j])], 1);
+  list_places(next, start, wsum, [](int, int) {});
+  int base = 0;
+  for (int w = 0; w < kListWaves; ++w) base += fewer[w];
+  if (tid < per && lo + tid <= vocab) offsets[lo + tid] = base + start[tid];
+  list_sort(found, first, cnt, next[wave], local_of, [&](int row, int d, int at) {
+    order[base + at] = row;
+    keys[base + at] = static_cast<int32_t>(lo) + d;
+  });
+}
+
+// ---- one launch for the shortest batches ----------------------------------------------
+// A workgroup owns the tokens v = range (mod ranges), ranges a power of two (so
+// that neighbouring, often equally frequent ids part), and `lanes` V columns. It
+// reads every token of the batch from L2, lists the rows of its own, sorts the
+// list (stable, by the token's number within the range: at most 256, one digit)
+// and sums each token's rows, `lanes` lanes per token; a token of many rows takes
+// all of the workgroup's lane groups. Few columns to a workgroup spread such a
+// token over more CUs, at the price of reading the tokens more often.
+constexpr int kDirectRows = 2048;  // of a batch at most
+
+template <typename T, typename I, int V>
+__global__ __launch_bounds__(kList) void direct_kernel(const T* __restrict__ dx, int64_t ld,
+                                                       const I* __restrict__ tokens, float scale,
+                                                       float* __restrict__ dE, int n, int64_t vocab, int D, int log_ranges,
+                                                       int lanes) {
+  __shared__ uint16_t found[kDirectRows + kList], rows[kDirectRows + kList];
+  __shared__ int next[kListWaves][kLocal];
+  __shared__ int start[kLocal + 1], many[kLocal], n_many;
+  __shared__ int wsum[kListWaves];
+  __shared__ float red[kList * V];
+  constexpr int kLong = 32;  // rows that a lane group sums by itself
+  const int tid = thread_x(), lane = tid & 63, wave = tid >> 6, blk = block_x();
+  const int ranges = 1 << log_ranges, range = blk & (ranges - 1), slice = blk >> log_ranges;
+  const int per_range = static_cast<int>((vocab + ranges - 1) >> log_ranges);
+  const int share = (n + kList - 1) / kList * 64, first = wave * share;
+  const int cnt = list_rows(
+      tokens, n, vocab, found, first, first + share < n ? first + share : n,
+      [&](int32_t k) { return k < vocab && (k & (ranges - 1)) == range; }, [](bool, int32_t) {});
+  for (int i = lane; i < kLocal; i += 64) next[wave][i] = 0;
+  if (tid == 0) n_many = 0;
+  __builtin_amdgcn_wave_barrier();
+  auto local_of = [&](int row) { return static_cast<int>(static_cast<int64_t>(tokens[row]) >> log_ranges); };
+  for (int j = lane; j < cnt; j += 64) atomicAdd(&next[wave][local_of(found[first + j])], 1);
+  list_places(next, start, wsum, [&](int k, int count) {
+    if (count > kLong) many[atomicAdd(&n_many, 1)] = k;  // (in any order: each token has a sum of its own)
+  });
+  list_sort(found, first, cnt, next[wave], local_of, [&](int row, int, int at) { rows[at] = static_cast<uint16_t>(row); });
   __syncthreads();
 
-  const int groups = 64 / lanes, grp = lane / lanes, c = slice * 64 * V + (lane & (lanes - 1)) * V;
-  const int kLong = 64 * groups;  // rows that a wave sums by itself
-  auto sum_rows = [&](int a, int b, float (&s)[V]) {
+  const int groups = kList / lanes, grp = tid / lanes, c = (slice * lanes + (tid & (lanes - 1))) * V;
+  auto sum_rows = [&](int a, int b, int step, float (&s)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) s[i] = 0.0f;
-    if (c < D) {
 #pragma unroll 8
-      for (int j = a + grp; j < b; j += groups) {
-        float x[V];
-        load_row<V>(dx + rows[j] * ld + c, x);
+    for (int j = a; j < b; j += step) {
+      float x[V];
+      load_row<V>(dx + rows[j] * ld + c, x);
 #pragma unroll
-        for (int i = 0; i < V; ++i) s[i] += x[i];
-      }
+      for (int i = 0; i < V; ++i) s[i] += x[i];
     }
-    for (int o = lanes; o < 64; o *= 2)
-#pragma unroll
-      for (int i = 0; i < V; ++i) s[i] += __shfl_xor(s[i], o);
   };
-  for (int k = wave; k < per_range; k += kDirectWaves) {
+  // the tokens of many rows, one after the other: rows dealt to the groups, the groups' sums added in order
+  for (int m = 0; m < n_many; ++m) {
+    const int k = many[m], a = start[k], b = start[k + 1];
     const int64_t v = (static_cast<int64_t>(k) << log_ranges) | range;
-    const int a = start[k], b = start[k + 1];
-    if (v >= vocab || b - a > kLong) continue;
     float s[V];
-    sum_rows(a, b, s);
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[i] *= scale;
-    if (grp == 0 && c < D) store_row<V>(dE + v * D + c, s);
-  }
-  for (int k = 0; k < per_range; ++k) {
-    const int a = start[k], b = start[k + 1];
-    if (b - a <= kLong) continue;
-    const int64_t v = (static_cast<int64_t>(k) << log_ranges) | range;
-    const int each = (b - a + kDirectWaves - 1) / kDirectWaves, w0 = a + wave * each;
-    float s[V];
-    sum_rows(w0 < b ? w0 : b, w0 + each < b ? w0 + each : b, s);
+    for (int i = 0; i < V; ++i) s[i] = 0.0f;
+    if (c < D) sum_rows(a + grp, b, groups, s);
 #pragma unroll
     for (int i = 0; i < V; ++i) red[tid * V + i] = s[i];
     __syncthreads();
-    if (wave == 0 && grp == 0 && c < D) {
-      for (int w = 1; w < kDirectWaves; ++w)
+    // by halves: 64 lanes' worth of groups and more fold in log2(groups) steps
+    for (int o = groups / 2; o > 0; o /= 2) {
+      if (grp < o) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) s[i] += red[(w * 64 + lane) * V + i];
+        for (int i = 0; i < V; ++i) red[tid * V + i] += red[(tid + o * lanes) * V + i];
+      }
+      __syncthreads();
+    }
+    if (grp == 0 && c < D) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) s[i] *= scale;
+      for (int i = 0; i < V; ++i) s[i] = red[tid * V + i] * scale;
       store_row<V>(dE + v * D + c, s);
     }
     __syncthreads();
   }
-}
-
-__global__ __launch_bounds__(kThreads) void zero_kernel(float* __restrict__ p, int64_t n, int gx) {
-  for (int64_t i = static_cast<int64_t>(block_x()) * kThreads + thread_x(); i < n; i += static_cast<int64_t>(gx) * kThreads)
-    p[i] = 0.0f;
+  if (c >= D) return;
+  for (int k = grp; k < per_range; k += groups) {
+    const int64_t v = (static_cast<int64_t>(k) << log_ranges) | range;
+    const int a = start[k], b = start[k + 1];
+    if (v >= vocab || b - a > kLong) continue;
+    float s[V];
+    sum_rows(a, b, 1, s);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] *= scale;
+    store_row<V>(dE + v * D + c, s);
+  }
 }
 
 constexpr int64_t kMaxCount = 0x7fffffff - 4096;  // places and steps past the last one stay in 32 bits
@@ -452,10 +591,20 @@ int digit_bits(int64_t V, int* passes) {
   return (bits + *passes - 1) / *passes;
 }
 
+// Keys of a workgroup where a plan is made in one launch, 0 where it is sorted:
+// every workgroup reads all tokens, so it is for at most kShortRows rows and
+// kShortReads token reads in all.
+constexpr int64_t kShortReads = int64_t{1} << 25;
+int short_plan_keys(int64_t T, int64_t V) {
+  if (T > kShortRows) return 0;
+  const int64_t per = V / 256 + 1 < kLocal ? V / 256 + 1 : kLocal;
+  return (V / per + 1) * T <= kShortReads ? static_cast<int>(per) : 0;
+}
+
 // Rows of a span: enough spans to fill the chip, few enough pieces to add.
 int span_rows(int64_t T) {
-  int R = 64;
-  while (R < 512 && T / R > 2048) R *= 2;
+  int R = 8;
+  while (R < kMaxSpan && T / R > 2048) R *= 2;
   return R;
 }
 
@@ -541,6 +690,16 @@ extern "C" int agpt_embed_plan(const void* tokens, int token_bits, int64_t T, in
     return invalid(what, "workspace smaller than agpt_embed_plan_workspace_bytes");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   int32_t *order = plan, *keys = plan + T, *offsets = plan + 2 * T;
+  if (const int per = short_plan_keys(T, V)) {
+    const dim3 grid(static_cast<unsigned>(V / per + 1));
+    if (token_bits == 32)
+      hipLaunchKernelGGL((short_plan_kernel<int32_t>), grid, dim3(kList), 0, st, static_cast<const int32_t*>(tokens),
+                         static_cast<int>(T), V, per, order, keys, offsets);
+    else
+      hipLaunchKernelGGL((short_plan_kernel<int64_t>), grid, dim3(kList), 0, st, static_cast<const int64_t*>(tokens),
+                         static_cast<int>(T), V, per, order, keys, offsets);
+    return launch_status(what);
+  }
   int passes;
   const int bits = digit_bits(V, &passes), digits = 1 << bits;
   if (T > 0) {
@@ -605,37 +764,42 @@ extern "C" int agpt_embed_bwd(const void* dx, int64_t ld_dx, const int32_t* plan
     return launch_status(what);
   }
   const int R = span_rows(T), spans = static_cast<int>((T + R - 1) / R);
-  const int64_t waves = (V + kWaves - 1) / kWaves;
-  if (waves + spans > 0x7fffffff) return invalid(what, "T and V too large together");
   const int32_t *order = plan, *keys = plan + T, *offsets = plan + 2 * T;
   const bool wide = wide_rows(D, ld_dx, es, dx, d_table);
   with_dtype(dtype, wide, [&](auto e, auto vc) {
     using E = decltype(e);
     constexpr int W = decltype(vc)::value;
-    hipLaunchKernelGGL((sums_kernel<E, W>), dim3(static_cast<unsigned>(spans + waves)), dim3(kThreads), 0, st,
+    const int lanes = lanes_for(D, W);
+    const int64_t blocks = spans + (V + kZeroRows - 1) / kZeroRows;  // far below 2^31
+    hipLaunchKernelGGL((sums_kernel<E, W>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st,
                        static_cast<const E*>(dx), ld_dx, order, keys, offsets, scale, d_table, workspace,
-                       static_cast<int32_t>(T), static_cast<int32_t>(V), D, R, spans, lanes_for(D, W));
+                       static_cast<int32_t>(T), static_cast<int32_t>(V), D, R, spans, lanes);
   });
   if (const int rc = launch_status(what)) return rc;
+  if (spans == 1) return AGPT_OK;  // no token goes over spans
   int lanes = 1;
   while (lanes < D && lanes < 128) lanes *= 2;
-  hipLaunchKernelGGL(join_kernel, dim3(spans), dim3(kJoin), 0, st, workspace, keys, offsets, scale, d_table,
-                     static_cast<int32_t>(T), static_cast<int32_t>(V), D, R, lanes);
+  const int each = (spans + 255) / 256;
+  hipLaunchKernelGGL(join_kernel, dim3((spans + each - 1) / each, (D + lanes - 1) / lanes), dim3(kJoin), 0, st, workspace,
+                     keys, offsets, scale, d_table, static_cast<int32_t>(T), static_cast<int32_t>(V), D, R, lanes, spans,
+                     each);
   return launch_status(what);
 }
 
 namespace {
 
-// The one-launch form: log2 of its ranges, or -1 where sorting first is taken.
-// Every workgroup reads all tokens, so it is for batches of at most kDirectRows
-// rows, and for at most kDirectReads token reads in all.
-constexpr int64_t kDirectRows = 16384, kDirectReads = int64_t{1} << 25;
-int direct_ranges(int64_t T, int64_t V, int D, int width) {
+// The one-launch form: log2 of its ranges, or -1 where a plan is made first.
+// Every workgroup reads all tokens, and one long token's rows are one workgroup's:
+// for at most kDirectRows rows and kShortReads token reads in all.
+int direct_ranges(int64_t T, int64_t V, int D, int width, int* lanes) {
   if (T < 1 || T > kDirectRows) return -1;
-  const int64_t slices = (D + 64 * width - 1) / (64 * width);
-  int lr = 0;
-  while ((static_cast<int64_t>(kLocal) << lr) < V || ((slices << lr) < 512 && (int64_t{1} << lr) < V)) ++lr;
-  return (slices << lr) * T <= kDirectReads ? lr : -1;
+  for (*lanes = 16; *lanes <= 64; *lanes *= 2) {  // the fewest columns that the reads allow
+    const int64_t slices = (D + *lanes * width - 1) / (*lanes * width);
+    int lr = 0;
+    while ((static_cast<int64_t>(kLocal) << lr) < V || ((slices << lr) < 512 && (int64_t{1} << lr) < V)) ++lr;
+    if ((slices << lr) * T <= kShortReads) return lr;
+  }
+  return -1;
 }
 
 }  // namespace
@@ -663,7 +827,8 @@ extern "C" int agpt_embed_bwd_tokens(const void* dx, int64_t ld_dx, const void* 
     return invalid(what, "workspace smaller than agpt_embed_bwd_tokens_workspace_bytes");
   const bool wide = wide_rows(D, ld_dx, es, dx, d_table);
   const int width = !wide ? 1 : (dtype == AGPT_DTYPE_F32 ? 4 : 8);
-  const int lr = direct_ranges(T, V, D, width);
+  int lanes;
+  const int lr = direct_ranges(T, V, D, width, &lanes);
   if (lr < 0) {
     int32_t* plan = static_cast<int32_t*>(workspace);
     int32_t* rest = plan + agpt_embed_plan_ints(T, V);
@@ -674,21 +839,15 @@ extern "C" int agpt_embed_bwd_tokens(const void* dx, int64_t ld_dx, const void* 
   with_dtype(dtype, wide, [&](auto e, auto vc) {
     using E = decltype(e);
     constexpr int W = decltype(vc)::value;
-    int lanes = 1;
-    while (lanes * W < D && lanes < 64) lanes *= 2;
-    const dim3 grid(static_cast<unsigned>(((D + 64 * W - 1) / (64 * W)) << lr));
-    auto go = [&](auto tok, auto cap) {
+    const dim3 grid(static_cast<unsigned>(((D + lanes * W - 1) / (lanes * W)) << lr));
+    auto go = [&](auto tok) {
       using I = decltype(tok);
-      hipLaunchKernelGGL((direct_kernel<E, I, W, decltype(cap)::value>), grid, dim3(kDirect), 0,
-                         static_cast<hipStream_t>(stream), static_cast<const E*>(dx), ld_dx, static_cast<const I*>(tokens),
-                         scale, d_table, static_cast<int>(T), V, D, lr, lanes);
+      hipLaunchKernelGGL((direct_kernel<E, I, W>), grid, dim3(kList), 0, static_cast<hipStream_t>(stream),
+                         static_cast<const E*>(dx), ld_dx, static_cast<const I*>(tokens), scale, d_table,
+                         static_cast<int>(T), V, D, lr, lanes);
     };
-    auto size = [&](auto tok) {
-      if (T <= 2048) go(tok, std::integral_constant<int, 2048>{});
-      else go(tok, std::integral_constant<int, kDirectRows>{});
-    };
-    if (token_bits == 32) size(int32_t{});
-    else size(int64_t{});
+    if (token_bits == 32) go(int32_t{});
+    else go(int64_t{});
   });
   return launch_status(what);
 }
