@@ -59,6 +59,40 @@ __device__ __forceinline__ void store_row(bf16_t* __restrict__ p, const float (&
   }
 }
 
+// V elements as they are in memory, loaded in one piece: what a row that is still
+// on its way takes in registers.
+template <typename T, int V>
+struct Raw {
+  static constexpr int kWords = V * static_cast<int>(sizeof(T)) / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T* __restrict__ p) {
+    if constexpr (kWords == 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else {
+      static_assert(kWords == 2, "8 or 16 bytes");
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x; w[1] = v.y;
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0u;
+  }
+  __device__ __forceinline__ void get(float (&x)[V]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; i += 2) {
+        x[i] = __uint_as_float(w[i / 2] << 16);
+        x[i + 1] = __uint_as_float(w[i / 2] & 0xffff0000u);
+      }
+    }
+  }
+};
+
 template <int kCtrl>
 __device__ __forceinline__ float dpp(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xf, 0xf, false));
