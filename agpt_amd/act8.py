@@ -12,7 +12,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _native
-from .block import _check_cuda, _dtype, _launch, _ptr, _rows, _stream
+from .block import _check_cuda, _dtype, _launch, _ptr, _rows
 
 BLOCK = 32  # columns of a row under one scale
 
@@ -45,8 +45,7 @@ def pack(x, relu: bool = False) -> Act8:
     lib = _native.attn_lib()
     codes = torch.empty(lib.agpt_act8_code_bytes(T, W), device=x.device, dtype=torch.uint8)
     scales = torch.empty(lib.agpt_act8_scale_bytes(T, W), device=x.device, dtype=torch.uint8)
-    _launch(x.device, lambda: lib.agpt_act8_pack(
-        _ptr(x), ld, dt, int(relu), _ptr(codes), _ptr(scales), T, W, _stream(x)))
+    _launch(x.device, lib.agpt_act8_pack, _ptr(x), ld, dt, int(relu), _ptr(codes), _ptr(scales), T, W)
     return Act8(codes, scales, T, W, bool(relu))
 
 
@@ -59,8 +58,8 @@ def unpack(kept: Act8, dtype=torch.float32, out=None):
     if out.shape != (kept.T, kept.W):
         raise ValueError("out must be shaped as the checkpoint")
     lib = _native.attn_lib()
-    _launch(kept.device, lambda: lib.agpt_act8_unpack(
-        _ptr(kept.codes), _ptr(kept.scales), int(kept.relu), _ptr(out), ld, dt, kept.T, kept.W, _stream(out)))
+    _launch(kept.device, lib.agpt_act8_unpack, _ptr(kept.codes), _ptr(kept.scales), int(kept.relu), _ptr(out), ld, dt, kept.T,
+            kept.W)
     return out
 
 
@@ -83,9 +82,8 @@ def wgrad(dy, kept: Act8, bias: bool = True):
     weight and bias from dy [T, out] (fp32 or bf16, rows may be strided) and its
     checkpointed input."""
     lib, dt, ld, T, out, ws, n, dw, db = _grads(dy, kept, bias)
-    _launch(dy.device, lambda: lib.agpt_act8_wgrad(
-        _ptr(dy), ld, dt, _ptr(kept.codes), _ptr(kept.scales), int(kept.relu), _ptr(dw), _ptr(db), _ptr(ws), n, T, out,
-        kept.W, _stream(dy)))
+    _launch(dy.device, lib.agpt_act8_wgrad, _ptr(dy), ld, dt, _ptr(kept.codes), _ptr(kept.scales), int(kept.relu), _ptr(dw),
+            _ptr(db), _ptr(ws), n, T, out, kept.W)
     return dw, db
 
 
@@ -100,7 +98,6 @@ def relu_wgrad(dh, h: Act8, kept: Act8, bias: bool = True):
         raise ValueError("dh must be shaped as h")
     lib, dt, ld, T, out, ws, n, dw, db = _grads(dh, kept, bias)
     masked = torch.empty(T, out, device=dh.device, dtype=dh.dtype)
-    _launch(dh.device, lambda: lib.agpt_act8_relu_wgrad(
-        _ptr(dh), ld, dt, _ptr(h.codes), _ptr(masked), _ptr(kept.codes), _ptr(kept.scales), int(kept.relu), _ptr(dw),
-        _ptr(db), _ptr(ws), n, T, out, kept.W, _stream(dh)))
+    _launch(dh.device, lib.agpt_act8_relu_wgrad, _ptr(dh), ld, dt, _ptr(h.codes), _ptr(masked), _ptr(kept.codes),
+            _ptr(kept.scales), int(kept.relu), _ptr(dw), _ptr(db), _ptr(ws), n, T, out, kept.W)
     return masked, dw, db

@@ -7,26 +7,35 @@ from __future__ import annotations
 
 import ctypes as C
 
+import torch
+
 from . import _native
 
 
 def _ptr(t):
-    return None if t is None else C.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
-def _stream(t) -> C.c_void_p:
-    import torch
-    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+def _stream(t) -> int:
+    return torch.cuda.current_stream(t.device).cuda_stream
 
 
-def _launch(device, call) -> None:
-    """Runs a native call with `device` current, and raises on its status."""
-    import torch
-    if device.index == torch.cuda.current_device():
-        _native.check(call())
+# The current stream's handle and the current device by themselves: torch.cuda's
+# own calls build objects around them, 3 us of a 10 us lookup of one token.
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
+def _launch(device, fn, *args) -> None:
+    """Calls fn(*args, the device's current stream) with `device` (a tensor's)
+    current, and raises on its status."""
+    i = device.index
+    if i == _current_device():
+        rc = fn(*args, _raw_stream(i))
     else:
         with torch.cuda.device(device):
-            _native.check(call())
+            rc = fn(*args, _raw_stream(i))
+    if rc:
+        _native.check(rc)
 
 
 def _check_cuda(name: str, t, device=None) -> None:
@@ -36,13 +45,14 @@ def _check_cuda(name: str, t, device=None) -> None:
         raise ValueError(f"{name} must be on {device}")
 
 
+_DTYPES = {torch.float32: _native.AGPT_DTYPE_F32, torch.bfloat16: _native.AGPT_DTYPE_BF16}
+
+
 def _dtype(name: str, t) -> int:
-    import torch
-    if t.dtype == torch.float32:
-        return _native.AGPT_DTYPE_F32
-    if t.dtype == torch.bfloat16:
-        return _native.AGPT_DTYPE_BF16
-    raise ValueError(f"{name} must be float32 or bfloat16")
+    dt = _DTYPES.get(t.dtype)
+    if dt is None:
+        raise ValueError(f"{name} must be float32 or bfloat16")
+    return dt
 
 
 def _rows(name: str, t) -> int:
@@ -71,7 +81,6 @@ def bias_rope_(x, bias=None, positions=None, cos_t=None, sin_t=None, n_heads: in
 
 def bias_rope_split(qkv, bias=None, positions=None, cos_t=None, sin_t=None, n_heads: int = 1):
     """qkv [T, 3D] -> contiguous (q, k, v) [T, D]: bias on all, RoPE on q, k."""
-    import torch
     if not qkv.is_cuda or not qkv.is_contiguous() or qkv.dim() != 2 or qkv.shape[1] % 3:
         raise ValueError("qkv must be a contiguous CUDA [T, 3D] tensor")
     T, D3 = qkv.shape
@@ -88,7 +97,6 @@ def bias_rope_split(qkv, bias=None, positions=None, cos_t=None, sin_t=None, n_he
 
 def _qk_args(qkv, wq, wk, bias, positions, cos_t, sin_t, n_heads, n_kv_heads):
     """Checks what the norm's two directions share; the row's head counts and sizes."""
-    import torch
     _check_cuda("qkv", qkv)
     dt, ld = _dtype("qkv", qkv), _rows("qkv", qkv)
     Hk = n_heads if n_kv_heads is None else n_kv_heads
@@ -121,12 +129,10 @@ def qk_norm_rope_split(qkv, wq, wk, bias=None, positions=None, cos_t=None, sin_t
     the rotation: qkv [T, (n_heads + 2 n_kv_heads) hd] (fp32 or bf16, rows may
     be strided) -> contiguous q [T, n_heads hd], k and v [T, n_kv_heads hd].
     wq, wk [hd] and bias are fp32; n_kv_heads None: as many as n_heads."""
-    import torch
     dt, ld, T, hd, Hk, seq = _qk_args(qkv, wq, wk, bias, positions, cos_t, sin_t, n_heads, n_kv_heads)
     q, k, v = (torch.empty(T, h * hd, device=qkv.device, dtype=qkv.dtype) for h in (n_heads, Hk, Hk))
-    _launch(qkv.device, lambda: _native.attn_lib().agpt_qk_norm_rope_split(
-        _ptr(qkv), ld, _ptr(bias), _ptr(wq), _ptr(wk), _ptr(positions), _ptr(cos_t), _ptr(sin_t), seq, T, n_heads, Hk, hd,
-        C.c_float(eps), dt, _ptr(q), _ptr(k), _ptr(v), _stream(qkv)))
+    _launch(qkv.device, _native.attn_lib().agpt_qk_norm_rope_split, _ptr(qkv), ld, _ptr(bias), _ptr(wq), _ptr(wk),
+            _ptr(positions), _ptr(cos_t), _ptr(sin_t), seq, T, n_heads, Hk, hd, eps, dt, _ptr(q), _ptr(k), _ptr(v))
     return q, k, v
 
 
@@ -136,7 +142,6 @@ def qk_norm_rope_split_bwd(dq, dk, dv, qkv, wq, wk, bias=None, positions=None, c
     of its outputs; weights' and bias' gradients are fp32 sums in a fixed order.
     cos_t None: dq and dk are gradients in front of the rotation already (as
     TrieAttention.backward returns them when it is given the tables)."""
-    import torch
     dt, ld, T, hd, Hk, seq = _qk_args(qkv, wq, wk, bias, positions, cos_t, sin_t, n_heads, n_kv_heads)
     for name, t, h in (("dq", dq, n_heads), ("dk", dk, Hk), ("dv", dv, Hk)):
         _check_cuda(name, t, qkv.device)
@@ -153,10 +158,9 @@ def qk_norm_rope_split_bwd(dq, dk, dv, qkv, wq, wk, bias=None, positions=None, c
     ws = torch.empty(n, device=qkv.device, dtype=torch.float32)
     dwq, dwk = (torch.empty(hd, device=qkv.device, dtype=torch.float32) for _ in range(2))
     db = torch.empty(qkv.shape[1], device=qkv.device, dtype=torch.float32) if bias is not None else None
-    _launch(qkv.device, lambda: lib.agpt_qk_norm_rope_split_bwd(
-        _ptr(dq), _ptr(dk), _ptr(dv), _ptr(qkv), ld, _ptr(bias), _ptr(wq), _ptr(wk), _ptr(positions), _ptr(cos_t),
-        _ptr(sin_t), seq, T, n_heads, Hk, hd, C.c_float(eps), dt, _ptr(out), ld_out, _ptr(dwq), _ptr(dwk), _ptr(db),
-        _ptr(ws), n, _stream(qkv)))
+    _launch(qkv.device, lib.agpt_qk_norm_rope_split_bwd, _ptr(dq), _ptr(dk), _ptr(dv), _ptr(qkv), ld, _ptr(bias),
+            _ptr(wq), _ptr(wk), _ptr(positions), _ptr(cos_t), _ptr(sin_t), seq, T, n_heads, Hk, hd, eps, dt, _ptr(out),
+            ld_out, _ptr(dwq), _ptr(dwk), _ptr(db), _ptr(ws), n)
     return out, dwq, dwk, db
 
 
@@ -176,7 +180,6 @@ def rmsprop_(params, grads, sq_avg, lr: float, beta: float, eps: float = 1e-8):
 def relu_bwd(dy, h):
     """Returns (dh, db): dh = dy where h > 0 else 0 ([T, width]), db = its
     column sum [width] (fixed order), in one pass."""
-    import torch
     for t in (dy, h):
         if not t.is_cuda or not t.is_contiguous() or t.dim() != 2 or t.dtype != torch.float32:
             raise ValueError("dy and h must be contiguous float32 CUDA [T, width] tensors")
@@ -195,7 +198,6 @@ def relu_bwd(dy, h):
 def norm_fwd(x, w, b=None, eps: float = 1e-5):
     """LayerNorm (b given) or RMSNorm of the rows of x [T, D]; returns
     (y, mean or None, rstd)."""
-    import torch
     T, D = x.shape
     y = torch.empty_like(x)
     rstd = torch.empty(T, device=x.device, dtype=torch.float32)
@@ -208,7 +210,6 @@ def norm_fwd(x, w, b=None, eps: float = 1e-5):
 def norm_bwd(dy, x, w, mean, rstd, layer: bool, dres=None):
     """Returns (dx, dw, db or None) of norm_fwd; dres [T, D] (a residual
     stream's gradient at x) is added into dx in the same pass."""
-    import torch
     T, D = x.shape
     if dres is not None and (not dres.is_cuda or not dres.is_contiguous() or dres.shape != x.shape):
         raise ValueError("dres must be a contiguous CUDA tensor shaped as x")

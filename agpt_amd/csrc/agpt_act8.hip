@@ -756,6 +756,7 @@ __global__ __launch_bounds__(kFoldThreads) void wgrad_fold_kernel(const float* _
 
 constexpr int kUnits = 2048;      // waves: two per SIMD
 constexpr int kMinRows = 64;      // of a chunk
+constexpr int kOneChunk = 256;    // rows that one chunk takes: the fold's launch costs as much as the steps it saves
 constexpr int kMaxWidth = 32768;
 
 struct Plan {
@@ -777,7 +778,7 @@ Plan plan_of(int64_t T, int out, int in, int wo) {
   const int64_t tiles = static_cast<int64_t>(p.tiles_o) * p.tiles_i;
   int64_t chunks = (wo ? kUnits / 8 : kUnits) / tiles;
   if (chunks > (T + kMinRows - 1) / kMinRows) chunks = (T + kMinRows - 1) / kMinRows;
-  if (chunks < 1) chunks = 1;
+  if (chunks < 1 || T <= kOneChunk) chunks = 1;
   p.chunk_rows = ((T + chunks - 1) / chunks + step - 1) / step * step;
   if (p.chunk_rows < step) p.chunk_rows = step;
   p.chunks = static_cast<int>((T + p.chunk_rows - 1) / p.chunk_rows);

@@ -7,12 +7,10 @@ give the same bytes.
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
 from . import _native
-from .block import _check_cuda, _dtype, _launch, _ptr, _rows, _stream
+from .block import _check_cuda, _dtype, _launch, _ptr, _rows
 
 _BITS = {torch.int32: 32, torch.int64: 64}
 
@@ -39,8 +37,7 @@ def embed_fwd(tokens, table, scale: float = 1.0, out=None):
         _check_cuda("out", out, table.device)
         if out.shape != (T, D) or out.dtype != table.dtype or not out.is_contiguous():
             raise ValueError("out must be a contiguous [T, D] tensor of the table's type")
-    _launch(table.device, lambda: _native.attn_lib().agpt_embed_fwd(
-        _ptr(table), _ptr(tokens), bits, C.c_float(scale), _ptr(out), T, V, D, dt, _stream(table)))
+    _launch(table.device, _native.attn_lib().agpt_embed_fwd, _ptr(table), _ptr(tokens), bits, scale, _ptr(out), T, V, D, dt)
     return out
 
 
@@ -58,8 +55,7 @@ class EmbedPlan:
         self.rows = torch.empty(lib.agpt_embed_plan_ints(self.T, self.vocab), device=self.device, dtype=torch.int32)
         n = lib.agpt_embed_plan_workspace_bytes(self.T, self.vocab)
         ws = torch.empty(n, device=self.device, dtype=torch.uint8)
-        _launch(self.device, lambda: lib.agpt_embed_plan(
-            _ptr(tokens), bits, self.T, self.vocab, _ptr(self.rows), _ptr(ws), n, _stream(tokens)))
+        _launch(self.device, lib.agpt_embed_plan, _ptr(tokens), bits, self.T, self.vocab, _ptr(self.rows), _ptr(ws), n)
 
 
 def embed_bwd(dx, tokens, vocab: int | None = None, scale: float = 1.0, out=None):
@@ -91,11 +87,10 @@ def embed_bwd(dx, tokens, vocab: int | None = None, scale: float = 1.0, out=None
     if plan is None:
         n = lib.agpt_embed_bwd_tokens_workspace_bytes(T, vocab, D)
         ws = torch.empty(n, device=device, dtype=torch.uint8)
-        _launch(device, lambda: lib.agpt_embed_bwd_tokens(
-            _ptr(dx), ld, _ptr(tokens), bits, C.c_float(scale), _ptr(out), _ptr(ws), n, T, vocab, D, dt, _stream(dx)))
+        _launch(device, lib.agpt_embed_bwd_tokens, _ptr(dx), ld, _ptr(tokens), bits, scale, _ptr(out), _ptr(ws), n, T, vocab,
+                D, dt)
         return out
     n = lib.agpt_embed_bwd_workspace_floats(T, D)
     ws = torch.empty(n, device=device, dtype=torch.float32)
-    _launch(device, lambda: lib.agpt_embed_bwd(
-        _ptr(dx), ld, _ptr(plan.rows), C.c_float(scale), _ptr(out), _ptr(ws), n, T, vocab, D, dt, _stream(dx)))
+    _launch(device, lib.agpt_embed_bwd, _ptr(dx), ld, _ptr(plan.rows), scale, _ptr(out), _ptr(ws), n, T, vocab, D, dt)
     return out
