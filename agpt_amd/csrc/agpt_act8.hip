@@ -640,6 +640,7 @@ __global__ __launch_bounds__(kShared, 2) void wgrad_shared_kernel(const T* __res
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[p][j][r] = 0.0f;
   auto multiply = [&](const uint4* a, const uint4* b) {
+    __builtin_amdgcn_s_setprio(2);  // over the preparation of the wave that shares the SIMD
     a += wo * kGroupA + l;
     b += 2 * wi * kGroupB + l;
 #pragma unroll
@@ -659,6 +660,7 @@ __global__ __launch_bounds__(kShared, 2) void wgrad_shared_kernel(const T* __res
                                                                 __builtin_bit_cast(bf16x8, fb[j]), acc[p][j], 0, 0, 0);
         }
     }
+    __builtin_amdgcn_s_setprio(0);
   };
   auto prepare = [&](int64_t t, Raw& w, int buf) {
 #pragma unroll
