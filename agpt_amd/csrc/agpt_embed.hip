@@ -460,12 +460,12 @@ __device__ __forceinline__ void list_sort(const uint16_t* found, int first, int 
 // A workgroup owns the keys lo .. lo + per - 1 (of 0 .. V). It reads every token
 // from L2, counts those below lo, which is where its own begin, and lists and
 // sorts its own: no workgroup waits for another.
-constexpr int kShortRows = 16384;
-template <typename I>
+constexpr int kShortRows = 32768;  // rows' numbers fit 16 bits
+template <typename I, int kCap>
 __global__ __launch_bounds__(kList) void short_plan_kernel(const I* __restrict__ tokens, int n, int64_t vocab, int per,
                                                            int32_t* __restrict__ order, int32_t* __restrict__ keys,
                                                            int32_t* __restrict__ offsets) {
-  __shared__ uint16_t found[kShortRows + kList];
+  __shared__ uint16_t found[kCap + kList];
   __shared__ int next[kListWaves][kLocal];
   __shared__ int start[kLocal + 1];
   __shared__ int wsum[kListWaves], fewer[kListWaves];
@@ -592,11 +592,13 @@ int digit_bits(int64_t V, int* passes) {
 }
 
 // Keys of a workgroup where a plan is made in one launch, 0 where it is sorted:
-// every workgroup reads all tokens, so it is for at most kShortRows rows and
-// kShortReads token reads in all.
+// every workgroup reads all tokens, so it is for at most kShortRows rows (half of
+// them where the sort is a single pass) and kShortReads token reads in all. Plan
+// and sums of rows of 128, one launch against sorting: 32K rows over 300 tokens
+// 39 and 50 us, over 50,000 59 and 60, over 65 36 and 28; 16K rows over 65 25 and 27.
 constexpr int64_t kShortReads = int64_t{1} << 25;
 int short_plan_keys(int64_t T, int64_t V) {
-  if (T > kShortRows) return 0;
+  if (T > (V < kDigits ? kShortRows / 2 : kShortRows)) return 0;
   const int64_t per = V / 256 + 1 < kLocal ? V / 256 + 1 : kLocal;
   return (V / per + 1) * T <= kShortReads ? static_cast<int>(per) : 0;
 }
@@ -692,12 +694,17 @@ extern "C" int agpt_embed_plan(const void* tokens, int token_bits, int64_t T, in
   int32_t *order = plan, *keys = plan + T, *offsets = plan + 2 * T;
   if (const int per = short_plan_keys(T, V)) {
     const dim3 grid(static_cast<unsigned>(V / per + 1));
-    if (token_bits == 32)
-      hipLaunchKernelGGL((short_plan_kernel<int32_t>), grid, dim3(kList), 0, st, static_cast<const int32_t*>(tokens),
-                         static_cast<int>(T), V, per, order, keys, offsets);
-    else
-      hipLaunchKernelGGL((short_plan_kernel<int64_t>), grid, dim3(kList), 0, st, static_cast<const int64_t*>(tokens),
-                         static_cast<int>(T), V, per, order, keys, offsets);
+    auto go = [&](auto tok, auto cap) {
+      using I = decltype(tok);
+      hipLaunchKernelGGL((short_plan_kernel<I, decltype(cap)::value>), grid, dim3(kList), 0, st,
+                         static_cast<const I*>(tokens), static_cast<int>(T), V, per, order, keys, offsets);
+    };
+    auto size = [&](auto tok) {  // (the smaller list leaves a CU room for three workgroups)
+      if (T <= 16384) go(tok, std::integral_constant<int, 16384>{});
+      else go(tok, std::integral_constant<int, kShortRows>{});
+    };
+    if (token_bits == 32) size(int32_t{});
+    else size(int64_t{});
     return launch_status(what);
   }
   int passes;

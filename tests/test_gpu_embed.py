@@ -73,7 +73,8 @@ def test_embed_fwd(gpu, T, V, D, dtype, bits, kind):
     (20_000, 3, 1500, "f32", 64, "skew"), (16_385, 1024, 96, "f32", 32, "skew"),
     (16_384, 1024, 96, "f32", 32, "skew"), (16_384, 5, 40, "bf16", 64, "one"), (2048, 300, 520, "f32", 64, "pad"),
     (2049, 300, 1040, "bf16", 32, "skew"), (300, 131_072, 8, "f32", 64, "skew"), (40, 1_000_000, 16, "f32", 64, "pad"),
-    (16_384, 400_000, 8, "f32", 64, "pad"), (511, 129, 3, "f32", 32, "skew")])
+    (65_536, 400, 24, "bf16", 32, "skew"), (65_537, 400, 24, "f32", 64, "pad"), (40_001, 70_000, 16, "f32", 64, "pad"),
+    (30_000, 65, 64, "f32", 32, "one"), (70_001, 131, 36, "f32", 32, "pad"), (16_384, 400_000, 8, "f32", 64, "pad"), (511, 129, 3, "f32", 32, "skew")])
 def test_embed_bwd(gpu, T, V, D, dtype, bits, kind):
     rng = np.random.default_rng(7 * T + V + D)
     tok = _tokens(rng, T, V, kind)
