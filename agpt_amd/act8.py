@@ -12,7 +12,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _native
-from .block import _check_cuda, _dtype, _launch, _ptr, _rows
+from .block import _check_apart, _check_cuda, _dtype, _launch, _ptr, _rows
 
 BLOCK = 32  # columns of a row under one scale
 
@@ -53,10 +53,12 @@ def unpack(kept: Act8, dtype=torch.float32, out=None):
     """The values [T, W] that a checkpoint stands for, exactly, in fp32 or bf16."""
     if out is None:
         out = torch.empty(kept.T, kept.W, device=kept.device, dtype=dtype)
-    _check_cuda("out", out, kept.device)
+    else:
+        _check_cuda("out", out, kept.device)
+        if out.shape != (kept.T, kept.W):
+            raise ValueError("out must be shaped as the checkpoint")
+        _check_apart("out", out, kept.codes, kept.scales)
     dt, ld = _dtype("out", out), _rows("out", out)
-    if out.shape != (kept.T, kept.W):
-        raise ValueError("out must be shaped as the checkpoint")
     lib = _native.attn_lib()
     _launch(kept.device, lib.agpt_act8_unpack, _ptr(kept.codes), _ptr(kept.scales), int(kept.relu), _ptr(out), ld, dt, kept.T,
             kept.W)

@@ -55,6 +55,23 @@ def _dtype(name: str, t) -> int:
     return dt
 
 
+def _check_f32(name: str, t, n: int, device) -> None:
+    if t.dtype != torch.float32 or t.numel() != n or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous float32 with {n} elements on {device}")
+
+
+def _check_apart(name: str, out, *inputs) -> None:
+    """Refuses an output that shares memory with an input."""
+    def span(t):  # bytes from its first to behind its last element
+        n = sum((s - 1) * d for s, d in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+        return t.data_ptr(), t.data_ptr() + n * t.element_size()
+    a, b = span(out)
+    for t in inputs:
+        c, d = span(t)
+        if a < d and c < b:
+            raise ValueError(f"{name} must not overlap an input")
+
+
 def _rows(name: str, t) -> int:
     """The row stride, in elements, of a 2-D tensor whose rows are contiguous."""
     if t.dim() == 2 and t.numel() == 0:
@@ -106,20 +123,20 @@ def _qk_args(qkv, wq, wk, bias, positions, cos_t, sin_t, n_heads, n_kv_heads):
     if width < 1 or width % (n_heads + 2 * Hk):
         raise ValueError("qkv's width must be a multiple of n_heads + 2 n_kv_heads")
     hd = width // (n_heads + 2 * Hk)
-    seq = 0
-    small = [("wq", wq, hd), ("wk", wk, hd)] + ([("bias", bias, width)] if bias is not None else [])
+    device, seq = qkv.device, 0
+    _check_f32("wq", wq, hd, device)
+    _check_f32("wk", wk, hd, device)
+    if bias is not None:
+        _check_f32("bias", bias, width, device)
     if cos_t is not None:
         if sin_t is None or positions is None:
             raise ValueError("the rotation needs cos_t, sin_t and positions")
         seq = cos_t.shape[0]
-        small += [("cos_t", cos_t, seq * hd), ("sin_t", sin_t, seq * hd)]
-        _check_cuda("positions", positions, qkv.device)
-        if positions.dtype != torch.int32 or positions.shape != (T,) or not positions.is_contiguous():
-            raise ValueError("positions must be a contiguous int32 [T] tensor")
-    for name, t, n in small:
-        _check_cuda(name, t, qkv.device)
-        if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous float32 with {n} elements")
+        _check_f32("cos_t", cos_t, seq * hd, device)
+        _check_f32("sin_t", sin_t, seq * hd, device)
+        if (positions.dtype != torch.int32 or positions.shape != (T,) or positions.device != device
+                or not positions.is_contiguous()):
+            raise ValueError(f"positions must be a contiguous int32 [T] tensor on {device}")
     return dt, ld, T, hd, Hk, seq
 
 
@@ -130,7 +147,9 @@ def qk_norm_rope_split(qkv, wq, wk, bias=None, positions=None, cos_t=None, sin_t
     be strided) -> contiguous q [T, n_heads hd], k and v [T, n_kv_heads hd].
     wq, wk [hd] and bias are fp32; n_kv_heads None: as many as n_heads."""
     dt, ld, T, hd, Hk, seq = _qk_args(qkv, wq, wk, bias, positions, cos_t, sin_t, n_heads, n_kv_heads)
-    q, k, v = (torch.empty(T, h * hd, device=qkv.device, dtype=qkv.dtype) for h in (n_heads, Hk, Hk))
+    q = torch.empty(T, n_heads * hd, device=qkv.device, dtype=qkv.dtype)
+    k = torch.empty(T, Hk * hd, device=qkv.device, dtype=qkv.dtype)
+    v = torch.empty_like(k)
     _launch(qkv.device, _native.attn_lib().agpt_qk_norm_rope_split, _ptr(qkv), ld, _ptr(bias), _ptr(wq), _ptr(wk),
             _ptr(positions), _ptr(cos_t), _ptr(sin_t), seq, T, n_heads, Hk, hd, eps, dt, _ptr(q), _ptr(k), _ptr(v))
     return q, k, v
@@ -149,9 +168,11 @@ def qk_norm_rope_split_bwd(dq, dk, dv, qkv, wq, wk, bias=None, positions=None, c
             raise ValueError(f"{name} must be a contiguous [T, {h * hd}] tensor of qkv's type")
     if out is None:
         out = torch.empty(T, qkv.shape[1], device=qkv.device, dtype=qkv.dtype)
-    _check_cuda("out", out, qkv.device)
-    if out.shape != qkv.shape or out.dtype != qkv.dtype:
-        raise ValueError("out must be shaped as qkv and of its type")
+    else:
+        _check_cuda("out", out, qkv.device)
+        if out.shape != qkv.shape or out.dtype != qkv.dtype:
+            raise ValueError("out must be shaped as qkv and of its type")
+        _check_apart("out", out, dq, dk, dv, qkv)
     ld_out = _rows("out", out)
     lib = _native.attn_lib()
     n = lib.agpt_qk_norm_workspace_floats(n_heads, Hk, hd)

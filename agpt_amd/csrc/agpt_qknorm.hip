@@ -399,7 +399,7 @@ bool with_kernel(const Launch& l, int dtype, Fn&& fn) {
 }
 
 int check_shape(const char* what, int64_t T, int64_t ld, int n_heads, int n_kv_heads, int head_dim, int dtype,
-                bool rope, int seq, int64_t C) {
+                bool rope, int seq, int64_t C, float eps) {
   if (T < 0 || n_heads < 1 || n_kv_heads < 1) return invalid(what, "T < 0, n_heads < 1 or n_kv_heads < 1");
   if (head_dim < 4 || head_dim > 256 || head_dim % 4 != 0) {
     char msg[160];
@@ -413,6 +413,7 @@ int check_shape(const char* what, int64_t T, int64_t ld, int n_heads, int n_kv_h
   if (ld % (dtype == AGPT_DTYPE_BF16 && head_dim % 8 == 0 ? 8 : 4) != 0)
     return invalid(what, "row stride must be a multiple of 4 elements (of 8 in bf16 where head_dim is)");
   if (rope && seq < 1) return invalid(what, "rope_seq_len < 1");
+  if (!(eps >= 0.0f)) return invalid(what, "eps must not be negative");
   return AGPT_OK;
 }
 
@@ -424,7 +425,8 @@ extern "C" int agpt_qk_norm_rope_split(const void* qkv, int64_t ld_qkv, const fl
                                        int head_dim, float eps, int dtype, void* q, void* k, void* v, void* stream) {
   const char* what = "agpt_qk_norm_rope_split";
   const int64_t C = (static_cast<int64_t>(n_heads) + 2 * static_cast<int64_t>(n_kv_heads)) * head_dim;
-  if (const int rc = check_shape(what, T, ld_qkv, n_heads, n_kv_heads, head_dim, dtype, cos_t != nullptr, rope_seq_len, C))
+  if (const int rc = check_shape(what, T, ld_qkv, n_heads, n_kv_heads, head_dim, dtype, cos_t != nullptr, rope_seq_len, C,
+                               eps))
     return rc;
   if (T == 0) return AGPT_OK;
   if (!qkv || !wq || !wk || !q || !k || !v || (cos_t && (!sin_t || !positions)))
@@ -460,7 +462,8 @@ extern "C" int agpt_qk_norm_rope_split_bwd(const void* dq, const void* dk, const
   const char* what = "agpt_qk_norm_rope_split_bwd";
   const int64_t C = (static_cast<int64_t>(n_heads) + 2 * static_cast<int64_t>(n_kv_heads)) * head_dim;
   for (const int64_t ld : {ld_qkv, ld_dqkv})
-    if (const int rc = check_shape(what, T, ld, n_heads, n_kv_heads, head_dim, dtype, cos_t != nullptr, rope_seq_len, C))
+    if (const int rc = check_shape(what, T, ld, n_heads, n_kv_heads, head_dim, dtype, cos_t != nullptr, rope_seq_len, C,
+                               eps))
       return rc;
   if (!wq || !wk || !dwq || !dwk || !workspace ||
       (T > 0 && (!dq || !dk || !dv || !qkv || !dqkv || (cos_t && (!sin_t || !positions)))))

@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .block import _check_cuda, _dtype, _launch, _ptr, _rows
+from .block import _check_apart, _check_cuda, _dtype, _launch, _ptr, _rows
 
 _BITS = {torch.int32: 32, torch.int64: 64}
 
@@ -37,6 +37,7 @@ def embed_fwd(tokens, table, scale: float = 1.0, out=None):
         _check_cuda("out", out, table.device)
         if out.shape != (T, D) or out.dtype != table.dtype or not out.is_contiguous():
             raise ValueError("out must be a contiguous [T, D] tensor of the table's type")
+        _check_apart("out", out, table, tokens)
     _launch(table.device, _native.attn_lib().agpt_embed_fwd, _ptr(table), _ptr(tokens), bits, scale, _ptr(out), T, V, D, dt)
     return out
 
@@ -83,6 +84,7 @@ def embed_bwd(dx, tokens, vocab: int | None = None, scale: float = 1.0, out=None
         _check_cuda("out", out, device)
         if out.shape != (vocab, D) or out.dtype != torch.float32 or not out.is_contiguous():
             raise ValueError("out must be a contiguous float32 [vocab, D] tensor")
+        _check_apart("out", out, dx, plan.rows if plan is not None else tokens)
     lib = _native.attn_lib()
     if plan is None:
         n = lib.agpt_embed_bwd_tokens_workspace_bytes(T, vocab, D)

@@ -231,7 +231,8 @@ def test_refuses(gpu):
     k, h = act8.pack(x), act8.pack(x, relu=True)
     for call in (lambda: act8.pack(x[:, :40]), lambda: act8.pack(x.half()), lambda: act8.pack(x[0]), lambda: act8.pack(x.t()),
                  lambda: act8.pack(x[:1].expand(4, 64)), lambda: act8.unpack(k, torch.float16),
-                 lambda: act8.unpack(k, out=x[:3]), lambda: act8.wgrad(x[:3], k), lambda: act8.wgrad(x.double(), k),
+                 lambda: act8.unpack(k, out=x[:3]),
+                 lambda: act8.unpack(k, out=k.codes[:256].view(torch.float32).view(1, 64).expand(4, 64)), lambda: act8.wgrad(x[:3], k), lambda: act8.wgrad(x.double(), k),
                  lambda: act8.wgrad(x.cpu(), k), lambda: act8.wgrad(x[:, :0], k), lambda: act8.relu_wgrad(x, k, k),
                  lambda: act8.relu_wgrad(x[:, :32], h, k), lambda: act8.relu_wgrad(x, h, act8.pack(x[:3]))):
         with pytest.raises(ValueError):

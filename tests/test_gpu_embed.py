@@ -163,6 +163,7 @@ def test_embed_refuses(gpu):
                  lambda: embed.embed_bwd(dx, t), lambda: embed.embed_bwd(dx, t, 0), lambda: embed.embed_bwd(dx.t(), t, 5),
                  lambda: embed.embed_bwd(dx, embed.EmbedPlan(t, 5), 6), lambda: embed.embed_bwd(dx.expand(4, 8)[:, :0], t, 5),
                  lambda: embed.embed_bwd(dx, t, 5, out=torch.zeros(5, 8, device=gpu, dtype=torch.bfloat16)),
-                 lambda: embed.embed_bwd(dx[:1].expand(4, 8), t, 5)):
+                 lambda: embed.embed_bwd(dx[:1].expand(4, 8), t, 5),
+                 lambda: embed.embed_fwd(t, E, out=E[:4]), lambda: embed.embed_bwd(dx, t, 4, out=dx)):
         with pytest.raises(ValueError):
             call()

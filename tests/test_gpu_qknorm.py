@@ -213,3 +213,10 @@ def test_qk_norm_refuses(gpu):
             block.qk_norm_rope_split_bwd(*dd, **s, n_heads=2, n_kv_heads=1)
     with pytest.raises(ValueError):
         block.qk_norm_rope_split(**s, n_heads=0)
+    for out in (s["qkv"], torch.empty(4, 64, device=gpu), torch.empty(5, 64, device=gpu).bfloat16()):  # overlaps; shape; type
+        with pytest.raises(ValueError):
+            block.qk_norm_rope_split_bwd(*d, **s, n_heads=2, n_kv_heads=1, out=out)
+    buf = torch.zeros(5 * 96, device=gpu)  # an output that begins inside dq
+    with pytest.raises(ValueError):
+        block.qk_norm_rope_split_bwd(buf[:160].view(5, 32), d[1], d[2], **s, n_heads=2, n_kv_heads=1,
+                                     out=buf[100:420].view(5, 64))

@@ -76,7 +76,7 @@ def test_embed_bwd_tokens_refuses(kw, part):
                                                       a["ws"], a["n"], a["T"], a["V"], a["D"], a["dtype"], None), BAD, part)
 
 
-QK = dict(qkv=P, ld=192, bias=P, wq=P, wk=P, pos=P, cos=P, sin=P, seq=32, T=3, H=2, Hk=1, hd=48, dtype=0, q=P, k=P, v=P)
+QK = dict(eps=1e-5, qkv=P, ld=192, bias=P, wq=P, wk=P, pos=P, cos=P, sin=P, seq=32, T=3, H=2, Hk=1, hd=48, dtype=0, q=P, k=P, v=P)
 
 
 @pytest.mark.parametrize("kw,code,part", [
@@ -86,17 +86,17 @@ QK = dict(qkv=P, ld=192, bias=P, wq=P, wk=P, pos=P, cos=P, sin=P, seq=32, T=3, H
     (dict(ld=194), BAD, "multiple of 4"), (dict(ld=196, dtype=1), BAD, "of 8"), (dict(seq=0), BAD, "rope_seq_len"),
     (dict(qkv=None), BAD, "null"), (dict(wq=None), BAD, "null"), (dict(v=None), BAD, "null"),
     (dict(sin=None), BAD, "null"), (dict(pos=None), BAD, "null"), (dict(qkv=P + 8), BAD, "16-byte"),
-    (dict(bias=P + 4), BAD, "16-byte")])
+    (dict(bias=P + 4), BAD, "16-byte"), (dict(eps=-1e-5), BAD, "eps"), (dict(eps=float("nan")), BAD, "eps")])
 def test_qk_norm_refuses(kw, code, part):
     a = dict(QK, **kw)
     lib = _native.attn_lib()
     _refuses(lib.agpt_qk_norm_rope_split(a["qkv"], a["ld"], a["bias"], a["wq"], a["wk"], a["pos"], a["cos"], a["sin"],
-                                         a["seq"], a["T"], a["H"], a["Hk"], a["hd"], C.c_float(1e-5), a["dtype"], a["q"],
+                                         a["seq"], a["T"], a["H"], a["Hk"], a["hd"], C.c_float(a["eps"]), a["dtype"], a["q"],
                                          a["k"], a["v"], None), code, part)
     n = lib.agpt_qk_norm_workspace_floats(2, 1, 48) + 10**9
     _refuses(lib.agpt_qk_norm_rope_split_bwd(a["q"], a["k"], a["v"], a["qkv"], a["ld"], a["bias"], a["wq"], a["wk"],
                                              a["pos"], a["cos"], a["sin"], a["seq"], a["T"], a["H"], a["Hk"], a["hd"],
-                                             C.c_float(1e-5), a["dtype"], P, a["ld"], P, P, P, P, n, None), code, part)
+                                             C.c_float(a["eps"]), a["dtype"], P, a["ld"], P, P, P, P, n, None), code, part)
 
 
 @pytest.mark.parametrize("kw,part", [(dict(ldd=100), "row stride"), (dict(n=10), "workspace"), (dict(ws=None), "null"),
@@ -106,7 +106,7 @@ def test_qk_norm_bwd_refuses(kw, part):
     a.update(kw)
     _refuses(_native.attn_lib().agpt_qk_norm_rope_split_bwd(
         P, P, P, a["qkv"], a["ld"], a["bias"], a["wq"], a["wk"], a["pos"], a["cos"], a["sin"], a["seq"], a["T"], a["H"],
-        a["Hk"], a["hd"], C.c_float(1e-5), a["dtype"], a["dx"], a["ldd"], a["dwq"], P, P, a["ws"], a["n"], None), BAD, part)
+        a["Hk"], a["hd"], C.c_float(a["eps"]), a["dtype"], a["dx"], a["ldd"], a["dwq"], P, P, a["ws"], a["n"], None), BAD, part)
 
 
 @pytest.mark.parametrize("kw,code,part", [
