@@ -237,3 +237,28 @@ def test_refuses(gpu):
                  lambda: act8.relu_wgrad(x[:, :32], h, k), lambda: act8.relu_wgrad(x, h, act8.pack(x[:3]))):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("T,out,W", [(50, 6, 32), (300, 70, 160)])
+def test_wgrad_by_differences(gpu, T, out, W):
+    """<dy, val·Wᵀ> is linear in W: with whole numbers that the checkpoint holds as
+    they are, every sum is exact and a difference over a step of 1 is the gradient."""
+    g = torch.Generator().manual_seed(T)
+    x = torch.randint(-8, 9, (T, W), generator=g).float()
+    x[:, ::32] = 64.0  # every block's scale is 1
+    dy = torch.randint(-4, 5, (T, out), generator=g).float()
+    k = act8.pack(x.to(gpu))
+    val = act8.unpack(k).double().cpu()
+    assert torch.equal(val, x.double())
+    dw, db = (t.double().cpu() for t in act8.wgrad(dy.to(gpu), k))
+    weight = torch.randint(-3, 4, (out, W), generator=g).double()
+
+    def f(w):
+        return float((dy.double() * (val @ w.T)).sum())
+    for o in range(0, out, 7):
+        for i in range(0, W, 13):
+            up, down = weight.clone(), weight.clone()
+            up[o, i] += 1
+            down[o, i] -= 1
+            assert float(dw[o, i]) == (f(up) - f(down)) / 2
+    assert torch.equal(db, dy.double().sum(0))

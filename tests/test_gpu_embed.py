@@ -167,3 +167,23 @@ def test_embed_refuses(gpu):
                  lambda: embed.embed_fwd(t, E, out=E[:4]), lambda: embed.embed_bwd(dx, t, 4, out=dx)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("T,V,D", [(90, 7, 12), (3000, 7, 12)])
+def test_embed_gradient_by_differences(gpu, T, V, D):
+    """<dx, x(E)> is linear in E: with small whole numbers every sum is exact and
+    a difference over a step of 1 is the gradient itself."""
+    g = torch.Generator().manual_seed(T)
+    tok = torch.randint(-1, V + 1, (T,), generator=g).to(gpu)
+    E = torch.randint(-4, 5, (V, D), generator=g).float().to(gpu)
+    dx = torch.randint(-4, 5, (T, D), generator=g).float().to(gpu)
+    got = embed.embed_bwd(dx, tok, V, 2.0)
+
+    def f(table):
+        return float((embed.embed_fwd(tok, table, 2.0).double() * dx.double()).sum())
+    for v in range(V):
+        for c in range(0, D, 5):
+            up, down = E.clone(), E.clone()
+            up[v, c] += 1
+            down[v, c] -= 1
+            assert float(got[v, c]) == (f(up) - f(down)) / 2
