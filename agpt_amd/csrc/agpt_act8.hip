@@ -3,8 +3,8 @@
 //
 // Packing and unpacking are HBM-bound: a lane packs 16 bytes of eight rows (eight
 // loads in flight), the lanes of 32 columns share their blocks' scales, and a
-// lane's codes are 32 consecutive bytes (64 in bf16). 2^20 rows of 512 fp32 in
-// about 480 us, 2.7 GB at 5.6 TB/s.
+// lane's codes are 32 consecutive bytes (64 in bf16). Packing 2^20 rows of 512
+// fp32 takes 519 us (2.7 GB at 5.2 TB/s), unpacking 300K 128 us (6.0 TB/s).
 //
 // The weight gradient dW[o][i] = sum_t dy[t][o] val[t][i] contracts over rows
 // that are far apart in memory. A matrix instruction takes from each lane
@@ -18,7 +18,12 @@
 //   an fp32 dy is cut into three bf16 parts by truncation, 8 + 8 + 8 bits,
 //   which add up to it exactly: three products at the bf16 rate instead of one
 //   at the fp32 rate, 1/16 of it.
-// Chunks leave partial tiles, folded in chunk order.
+// Chunks leave partial tiles, folded in chunk order. Behind a ReLU (2^20 rows of
+// 512, input 128) HBM bounds it: 969 us, 5.0 GB at 5.1 TB/s. The wider layers'
+// form below is bound by the matrix units: 128 x 512 over 2^20 rows in 339-358 us,
+// 412 GFLOP of bf16 products at 1.15-1.2 PFLOP/s, where a library product of 8192^3
+// reaches 1.14; 1000 x 1024 over 64K rows of bf16 in 173-205 us, 0.66-0.78, with
+// LDS traffic beside it (operands out of it at three quarters of its rate).
 
 #include "rows.h"
 #include "../../include/agpt_act8.h"
@@ -796,8 +801,40 @@ __global__ __launch_bounds__(kFoldThreads) void wgrad_fold_kernel(const float* _
   }
 }
 
+// The fold of a large dW over few chunks: a thread per four columns, all chunks'
+// loads in flight, and db by the last workgroups.
+__global__ __launch_bounds__(kThreads) void wgrad_add_kernel(const float* __restrict__ part, int64_t n,
+                                                             const float* __restrict__ part_b, int64_t ldb, int chunks,
+                                                             int out, float* __restrict__ dw, float* __restrict__ db,
+                                                             int wblocks) {
+  const int blk = block_x();
+  if (blk < wblocks) {
+    const int64_t c = (static_cast<int64_t>(blk) * kThreads + thread_x()) * 4;
+    if (c >= n) return;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 16
+    for (int q = 0; q < chunks; ++q) {
+      const float4 v = *reinterpret_cast<const float4*>(part + q * n + c);
+      a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+    }
+    *reinterpret_cast<float4*>(dw + c) = a;
+  } else {
+    const int c = (blk - wblocks) * kThreads + thread_x();
+    if (c >= out) return;
+    float a = 0.0f;
+#pragma unroll 16
+    for (int q = 0; q < chunks; ++q) a += part_b[q * ldb + c];
+    db[c] = a;
+  }
+}
+
 constexpr int kUnits = 2048;      // waves: two per SIMD
 constexpr int kMinRows = 64;      // of a chunk
+// Where a thread per four columns folds the chunks: enough threads to fill the
+// chip, few enough loads each (1024 x 1000 over 16 chunks: 41 us by slots of rows,
+// of which 48 of 64 idle, 11 so).
+constexpr int64_t kAddWidth = int64_t{1} << 18;
+constexpr int kAddChunks = 64;
 constexpr int kOneChunk = 256;    // rows that one chunk takes: the fold's launch costs as much as the steps it saves
 constexpr int kMaxWidth = 32768;
 
@@ -895,6 +932,12 @@ int wgrad(const char* what, const void* dy, int64_t ld, int dtype, const uint8_t
   else kinds(bf16_t{});
   if (const int rc = launch_status(what)) return rc;
   if (direct) return AGPT_OK;
+  if (n >= kAddWidth && p.chunks <= kAddChunks) {
+    const int wblocks = static_cast<int>((n / 4 + kThreads - 1) / kThreads), bblocks = db ? (out + kThreads - 1) / kThreads : 0;
+    hipLaunchKernelGGL(wgrad_add_kernel, dim3(wblocks + bblocks), dim3(kThreads), 0, st, part, n, part_b, p.db_ld, p.chunks,
+                       out, dw, db, wblocks);
+    return launch_status(what);
+  }
   const int wblocks = static_cast<int>((n + 63) / 64), bblocks = db ? (out + 63) / 64 : 0;
   hipLaunchKernelGGL(wgrad_fold_kernel, dim3(wblocks + bblocks), dim3(kFoldThreads), 0, st, part, n, part_b, p.db_ld,
                      p.chunks, out, dw, db, wblocks);

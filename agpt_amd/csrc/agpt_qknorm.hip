@@ -14,6 +14,10 @@
 // rows (or, for wide rows, part of the heads of one: grid y), and walk the
 // rows grid-strided. dw and dbias leave as one partial row per workgroup and
 // are folded in a fixed order.
+//
+// 2^20 rows of 8 + 16 heads x 16 fp32: forward 600 us (3.2 GB at 5.4 TB/s), backward
+// 845 + 11 (4.8 GB at 5.7); 32K rows of 32 + 16 heads x 128 bf16: backward 232 + 14
+// (1.2 GB at 5.2 TB/s).
 
 #include "rows.h"
 #include "../../include/agpt_block.h"

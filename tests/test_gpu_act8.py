@@ -140,7 +140,8 @@ def _check_wgrad(dy, k, val, bias=True):
     (130, 64, 96, "bf16", False), (257, 1000, 1024, "bf16", True), (500, 17, 32, "bf16", False), (15, 200, 288, "bf16", True),
     (16, 64, 128, "f32", True), (17, 66, 64, "f32", False), (4100, 130, 256, "f32", False), (33, 7, 2048, "f32", False),
     (70, 201, 160, "f32", False), (95, 333, 288, "bf16", True), (64, 127, 192, "bf16", False), (31, 128, 160, "f32", True),
-    (33, 600, 1312, "f32", False), (3000, 128, 256, "bf16", False)])
+    (33, 600, 1312, "f32", False), (3000, 128, 256, "bf16", False), (600, 520, 512, "f32", False),
+    (700, 1023, 288, "bf16", True)])
 def test_wgrad(gpu, T, out, W, dtype, relu):
     rng = np.random.default_rng(T + 3 * out + W)
     k = act8.pack(_x(rng, T, W, "f32", relu).to(gpu), relu=relu)
