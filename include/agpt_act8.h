@@ -56,8 +56,9 @@ int agpt_act8_unpack(const uint8_t* codes, const uint8_t* scales, int relu, void
  * dy [T, out] of `dtype`, row stride ld_dy elements; the checkpoint is [T, in];
  * dw and db fp32, written whole (db NULL: not formed). An fp32 dy enters the
  * bf16 matrix products as three parts that add up to it exactly, so nothing of
- * it is rounded (a part below 2^-126 may count as zero); the sums are fp32 in a fixed order. A dy that is not finite
- * makes the results that it enters infinite or NaN. workspace: at least
+ * it is rounded (a part below 2^-126 may count as zero); the sums are fp32 in a
+ * fixed order. A dy that is not finite makes the results that it enters
+ * infinite or NaN. workspace: at least
  * agpt_act8_wgrad_workspace_floats(T, out, in) floats, 16-byte aligned, as dw
  * and db are. */
 int64_t agpt_act8_wgrad_workspace_floats(int64_t T, int out_width, int in_width);
