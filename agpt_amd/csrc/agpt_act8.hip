@@ -231,8 +231,13 @@ struct Held {
   uint4 h0, h1;
 };
 
-// kPair: columns 2l and 2l + 1 in one load (dy aligned to the pair, an even
-// width); otherwise columns l and l + 32.
+// Two columns of a row in one load, at the alignment of one (which global loads
+// do without): rows of an odd stride or base need no form of their own.
+typedef uint32_t pair_f32 __attribute__((ext_vector_type(2), aligned(4)));
+typedef uint32_t pair_bf16 __attribute__((aligned(2)));
+
+// kPair: columns 2l and 2l + 1 in one load; otherwise (a width of 1)
+// columns l and l + 32.
 template <typename T, bool kPair, bool kRelu>
 __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(const T* __restrict__ dy, const uint8_t* __restrict__ hc,
                                                             T* __restrict__ dh, const uint8_t* __restrict__ codes,
@@ -257,7 +262,9 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(const T* __restrict_
   const int64_t blocks = (g.rows + kRows - 1) / kRows;
   // A column past the edge is read as the last one: it only reaches entries of
   // dW, db and dh that are not written.
-  const int ca = ina ? oa : g.out - (kPair ? 2 : 1), cb = inb ? ob : g.out - 1, cq = inq ? quad : quads - 1;
+  // The last of an odd number of columns comes as the second of a pair.
+  const bool second = kPair && oa == g.out - 1;
+  const int ca = ina && !second ? oa : g.out - (kPair ? 2 : 1), cb = inb ? ob : g.out - 1, cq = inq ? quad : quads - 1;
   const uint32_t off_a = static_cast<uint32_t>(half * kRows * g.ld + ca) * sizeof(T);
   const uint32_t off_b = static_cast<uint32_t>(half * kRows * g.ld + cb) * sizeof(T);
   const uint32_t off_d = static_cast<uint32_t>(half * kRows * g.out + ca) * sizeof(T);
@@ -277,14 +284,14 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(const T* __restrict_
 
   auto row = [&](const char* p, Held<T>& w, int r) {
     if constexpr (sizeof(T) == 4 && kPair) {
-      const uint2 v = *reinterpret_cast<const uint2*>(p + off_a);
+      const pair_f32 v = *reinterpret_cast<const pair_f32*>(p + off_a);
       w.a[r][0] = v.x;
       w.a[r][1] = v.y;
     } else if constexpr (sizeof(T) == 4) {
       w.a[r][0] = *reinterpret_cast<const uint32_t*>(p + off_a);
       w.a[r][1] = *reinterpret_cast<const uint32_t*>(p + off_b);
     } else if constexpr (kPair) {
-      w.a[r][0] = *reinterpret_cast<const uint32_t*>(p + off_a);
+      w.a[r][0] = *reinterpret_cast<const pair_bf16*>(p + off_a);
     } else {
       w.a[r][0] = *reinterpret_cast<const uint16_t*>(p + off_a) |
                   static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + off_b)) << 16;
@@ -324,6 +331,13 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(const T* __restrict_
   };
 
   auto step = [&](int64_t t, Held<T>& w) {
+    if constexpr (kPair && !kRelu) {
+      if (g.out & 1) {
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+          w.a[r][0] = !second ? w.a[r][0] : (sizeof(T) == 4 ? w.a[r][sizeof(T) == 4 ? 1 : 0] : w.a[r][0] >> 16);
+      }
+    }
     if constexpr (kRelu) {
       const uint32_t h[kRows] = {w.h0.x, w.h0.y, w.h0.z, w.h0.w, w.h1.x, w.h1.y, w.h1.z, w.h1.w};
       const int sh = (l & 1) * 16;
@@ -463,7 +477,7 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(const T* __restrict_
 // (eight rows of a column as bf16), written and read without bank conflicts.
 constexpr int kShared = 512, kSRows = 32, kOctets = kSRows / kRows;
 
-template <typename T, int WO, bool kPair, bool kRelu>
+template <typename T, int WO, bool kRelu>
 __global__ __launch_bounds__(kShared, 2) void wgrad_shared_kernel(const T* __restrict__ dy, const uint8_t* __restrict__ hc,
                                                                   T* __restrict__ dh, const uint8_t* __restrict__ codes,
                                                                   const uint8_t* __restrict__ scales,
@@ -471,7 +485,9 @@ __global__ __launch_bounds__(kShared, 2) void wgrad_shared_kernel(const T* __res
                                                                   int64_t db_ld, Grad g, int grid) {
   constexpr int WI = 8 / WO, kParts = sizeof(T) == 4 ? 3 : 1;
   constexpr int kGroupA = kOctets * kParts * 2 * 32, kGroupB = kOctets * 2 * 32;  // uint4 each
-  // A wave's jobs of eight rows: of dy with two columns a lane (kPair) or one, of the codes with two.
+  // A wave's jobs of eight rows: of dy with two columns a lane (kPair) or, where that would leave waves without, one;
+  // of the codes with two.
+  constexpr bool kPair = WO == 4;
   constexpr int kCols = kPair ? 2 : 1, kJobsA = WO / (2 * kCols), kJobsB = WI / 2;
   __shared__ uint4 sa[2][WO * kGroupA];
   __shared__ uint4 sb[2][2 * WI * kGroupB];
@@ -490,6 +506,7 @@ __global__ __launch_bounds__(kShared, 2) void wgrad_shared_kernel(const T* __res
 
   // This wave's share of the preparation. A column past the edge is read as the
   // last one: it only reaches entries of dW, db and dh that are not written.
+  // The last of an odd number comes as the second of a pair.
   int ga[kJobsA], octa[kJobsA], cola[kJobsA];
   uint32_t off_a[kJobsA], off_d[kJobsA], off_h[kJobsA];
 #pragma unroll
@@ -498,7 +515,7 @@ __global__ __launch_bounds__(kShared, 2) void wgrad_shared_kernel(const T* __res
     ga[q] = kPair ? job >> 1 : job >> 2;
     octa[q] = kPair ? 2 * (job & 1) + half : job & 3;
     cola[q] = o0 + 64 * ga[q] + (kPair ? 2 * l : lane);
-    const int c = cola[q] < g.out ? cola[q] : g.out - kCols;
+    const int c = cola[q] + kCols <= g.out ? cola[q] : g.out - kCols;
     off_a[q] = static_cast<uint32_t>(octa[q] * kRows * g.ld + c) * sizeof(T);
     off_d[q] = static_cast<uint32_t>(octa[q] * kRows * g.out + c) * sizeof(T);
     off_h[q] = static_cast<uint32_t>(octa[q] * (g.out / 4) + c / 4) * (4 * kRows);
@@ -535,11 +552,13 @@ __global__ __launch_bounds__(kShared, 2) void wgrad_shared_kernel(const T* __res
     auto row = [&](int q, int r) {
       const char* p = pa + r * step + off_a[q];
       if constexpr (sizeof(T) == 4 && kPair) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        const pair_f32 v = *reinterpret_cast<const pair_f32*>(p);
         w.a[q][r][0] = v.x;
         w.a[q][r][1] = v.y;
-      } else if constexpr (sizeof(T) == 4 || kPair) {
+      } else if constexpr (sizeof(T) == 4) {
         w.a[q][r][0] = *reinterpret_cast<const uint32_t*>(p);
+      } else if constexpr (kPair) {
+        w.a[q][r][0] = *reinterpret_cast<const pair_bf16*>(p);
       } else {
         w.a[q][r][0] = *reinterpret_cast<const uint16_t*>(p);
       }
@@ -588,6 +607,12 @@ __global__ __launch_bounds__(kShared, 2) void wgrad_shared_kernel(const T* __res
 
   auto put_a = [&](int64_t t, Held& w, int q, uint4* to_lds) {
     auto& ra = w.a[q];
+    if constexpr (kPair && !kRelu) {
+      const bool second = cola[q] == g.out - 1;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+        ra[r][0] = !second ? ra[r][0] : (sizeof(T) == 4 ? ra[r][sizeof(T) == 4 ? 1 : 0] : ra[r][0] >> 16);
+    }
     if constexpr (kRelu) {
       const uint32_t h[kRows] = {w.h[q][0].x, w.h[q][0].y, w.h[q][0].z, w.h[q][0].w,
                                  w.h[q][1].x, w.h[q][1].y, w.h[q][1].z, w.h[q][1].w};
@@ -717,8 +742,8 @@ __global__ __launch_bounds__(kShared, 2) void wgrad_shared_kernel(const T* __res
   // Step n is multiplied from buffer n & 1 while step n + 1 is prepared and the
   // rows of the next kAhead steps are on their way: two where the registers hold
   // them (64K rows of 1024 x 1000 bf16 208 -> 179 us for one to two), one behind
-  // a ReLU and with two jobs a wave.
-  constexpr int kAhead = kRelu || kJobsA > 1 ? 1 : 2;
+  // a ReLU.
+  constexpr int kAhead = kRelu ? 1 : 2;
   const int steps = static_cast<int>((t1 - t0 + kSRows - 1) / kSRows);
   auto at = [&](int n) { return t0 + static_cast<int64_t>(n) * kSRows; };
   Held w0, w1;
@@ -894,7 +919,6 @@ int wgrad(const char* what, const void* dy, int64_t ld, int dtype, const uint8_t
     return invalid(what, "codes, scales, dw, db and workspace must be 16-byte aligned");
   if (!aligned(dy, es)) return invalid(what, "dy is not aligned to its elements");
   if (ld > (1 << 26)) return agpt_internal_set_error(AGPT_ERR_UNSUPPORTED, "agpt_act8: row strides above 2^26 are not supported");
-  const bool pair = out % 2 == 0 && ld % 2 == 0 && aligned(dy, 2 * es);
   const Plan p = plan_of(T, out, in, shared_wo(out, in));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t n = static_cast<int64_t>(out) * in;
@@ -909,23 +933,21 @@ int wgrad(const char* what, const void* dy, int64_t ld, int dtype, const uint8_t
     hipLaunchKernelGGL((wgrad_kernel<E, decltype(pc)::value, decltype(rc)::value>), grid, dim3(kThreads), 0, st,
                        static_cast<const E*>(dy), hc, static_cast<E*>(dh), codes, scales, part, part_b, p.db_ld, g);
   };
-  auto shared = [&](auto e, auto wc, auto pc, auto rc) {
+  auto shared = [&](auto e, auto wc, auto rc) {
     using E = decltype(e);
     const int n = static_cast<int>((units + 7) / 8 * 8);
-    hipLaunchKernelGGL((wgrad_shared_kernel<E, decltype(wc)::value, decltype(pc)::value, decltype(rc)::value>), dim3(n),
-                       dim3(kShared), 0, st, static_cast<const E*>(dy), hc, static_cast<E*>(dh), codes, scales, part, part_b,
-                       p.db_ld, g, n);
+    hipLaunchKernelGGL((wgrad_shared_kernel<E, decltype(wc)::value, decltype(rc)::value>), dim3(n), dim3(kShared), 0, st,
+                       static_cast<const E*>(dy), hc, static_cast<E*>(dh), codes, scales, part, part_b, p.db_ld, g, n);
   };
   using W2 = std::integral_constant<int, 2>;
   using W4 = std::integral_constant<int, 4>;
   auto kinds = [&](auto e) {
-    if (p.wo == 2 && hc) shared(e, W2{}, std::false_type{}, std::true_type{});
-    else if (p.wo == 2) shared(e, W2{}, std::false_type{}, std::false_type{});
-    else if (p.wo == 4 && hc) shared(e, W4{}, std::true_type{}, std::true_type{});
-    else if (p.wo == 4 && pair) shared(e, W4{}, std::true_type{}, std::false_type{});
-    else if (p.wo == 4) shared(e, W4{}, std::false_type{}, std::false_type{});
+    if (p.wo == 2 && hc) shared(e, W2{}, std::true_type{});
+    else if (p.wo == 2) shared(e, W2{}, std::false_type{});
+    else if (p.wo == 4 && hc) shared(e, W4{}, std::true_type{});
+    else if (p.wo == 4) shared(e, W4{}, std::false_type{});
     else if (hc) go(e, std::true_type{}, std::true_type{});
-    else if (pair) go(e, std::true_type{}, std::false_type{});
+    else if (out > 1) go(e, std::true_type{}, std::false_type{});
     else go(e, std::false_type{}, std::false_type{});
   };
   if (dtype == AGPT_DTYPE_F32) kinds(float{});
