@@ -868,10 +868,19 @@ struct Plan {
   int tiles_o, tiles_i, chunks;
   int64_t chunk_rows, db_ld;
 };
-// Shared operands where dW is wider than a wave's tile in both directions.
+// Shared operands where dW is wider than a wave's tile in both directions and
+// fills enough of the shared tile: one of those costs what kSharedTile of a wave's
+// do (2^18 fp32 rows: 95 us a tile against 15.5). Measured on both sides of it, fp32
+// and bf16 us, a wave alone | shared: 384 from 384 columns 285, 174 | 368, 183 (18
+// tiles | 4: alone); 128 from 256 77, 50 | 95, 61 (4 | 1: alone); 129 from 256 96, 66
+// | 99, 57 (6 | 1: shared); 200 from 256 132, 75 | 110, 65 (8 | 1: shared).
+constexpr int kSharedTile = 6;
 int shared_wo(int out, int in) {
   if (out <= kTileO || in <= kTileI) return 0;
-  return out <= 2 * kTileO ? 2 : 4;
+  const int wo = out <= 2 * kTileO ? 2 : 4, to = kTileO * wo, ti = kTileI * (8 / wo);
+  const int alone = ((out + kTileO - 1) / kTileO) * ((in + kTileI - 1) / kTileI);
+  const int tiles = ((out + to - 1) / to) * ((in + ti - 1) / ti);
+  return alone < kSharedTile * tiles ? 0 : wo;
 }
 Plan plan_of(int64_t T, int out, int in, int wo) {
   Plan p;

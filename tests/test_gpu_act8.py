@@ -150,6 +150,40 @@ def test_wgrad(gpu, T, out, W, dtype, relu):
     _check_wgrad(dy, k, val, bias=out != 33)
 
 
+@pytest.mark.parametrize("T,out,W,dtype,ld,shift", [
+    (70, 67, 480, "f32", 67, 0), (333, 120, 512, "bf16", 131, 3), (95, 190, 224, "bf16", 191, 1), (601, 129, 256, "f32", 133, 2),
+    (47, 255, 416, "f32", 256, 0), (1025, 300, 256, "bf16", 301, 5), (513, 97, 224, "f32", 99, 1)])
+def test_wgrad_partly_filled_tiles(gpu, T, out, W, dtype, ld, shift):
+    """Widths on both sides of the rule that shares operands between waves, under
+    odd strides and shifts; what stands around the rows does not enter."""
+    rng = np.random.default_rng(T + out)
+    k = act8.pack(_x(rng, T, W, "f32", False).to(gpu))
+    val = act8.unpack(k).double().cpu().numpy()
+    flat = torch.full((T * ld + shift + 8,), float("nan"), dtype=DT[dtype])
+    torch.as_strided(flat, (T, out), (ld, 1), shift).copy_(_x(rng, T, out, dtype, False))
+    _check_wgrad(torch.as_strided(flat.to(gpu), (T, out), (ld, 1), shift), k, val)
+
+
+def test_two_streams_at_once(gpu):
+    """Calls that overlap on two streams have workspaces of their own."""
+    rng = np.random.default_rng(12)
+    T, out, W = 20000, 200, 256
+    ks = [act8.pack(_x(rng, T, W, "f32", False).to(gpu)) for _ in range(2)]
+    dys = [_x(rng, T, out, "f32", False).to(gpu) for _ in range(2)]
+    want = [act8.wgrad(d, k) for d, k in zip(dys, ks)]
+    streams = [torch.cuda.Stream(gpu) for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(act8.wgrad(dys[i], ks[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for dw, db in got[i]:
+            assert torch.equal(dw, want[i][0]) and torch.equal(db, want[i][1])
+
+
 def test_wgrad_keeps_all_of_fp32(gpu):
     """Every bit of an fp32 dy enters: against 1 + k 2^-23 in one row, whose
     products with small whole values are exact in fp32."""
