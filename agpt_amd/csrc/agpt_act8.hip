@@ -927,7 +927,8 @@ int wgrad(const char* what, const void* dy, int64_t ld, int dtype, const uint8_t
   if (!aligned(codes, 16) || !aligned(scales, 16) || !aligned(dw, 16) || !aligned(db, 16) || !aligned(ws, 16))
     return invalid(what, "codes, scales, dw, db and workspace must be 16-byte aligned");
   if (!aligned(dy, es)) return invalid(what, "dy is not aligned to its elements");
-  if (ld > (1 << 26)) return agpt_internal_set_error(AGPT_ERR_UNSUPPORTED, "agpt_act8: row strides above 2^26 are not supported");
+  // a lane's offset from the step's first row, at most 24 rows and a width of 4 bytes, stays in 32 bits
+  if (ld > (1 << 25)) return agpt_internal_set_error(AGPT_ERR_UNSUPPORTED, "agpt_act8: row strides above 2^25 are not supported");
   const Plan p = plan_of(T, out, in, shared_wo(out, in));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t n = static_cast<int64_t>(out) * in;

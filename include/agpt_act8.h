@@ -53,7 +53,7 @@ int agpt_act8_unpack(const uint8_t* codes, const uint8_t* scales, int relu, void
 
 /* Weight and bias gradient of a linear layer whose input was checkpointed:
  *   dw [out, in] = sum over t of dy[t, :] ^T value[t, :],   db [out] = sum over t of dy[t, :]
- * dy [T, out] of `dtype`, row stride ld_dy elements; the checkpoint is [T, in];
+ * dy [T, out] of `dtype`, row stride ld_dy (up to 2^25) elements; the checkpoint is [T, in];
  * dw and db fp32, written whole (db NULL: not formed). An fp32 dy enters the
  * bf16 matrix products as three parts that add up to it exactly, so nothing of
  * it is rounded (a part below 2^-126 may count as zero); the sums are fp32 in a

@@ -142,6 +142,15 @@ def test_act8_wgrad_refuses(kw, code, part):
              "" if part == "width" else part)
 
 
+@pytest.mark.parametrize("ld", [2**25 + 4, 2**26, 2**32 + 64])
+def test_act8_wgrad_refuses_strides_past_its_offsets(ld):
+    """24 rows of 2^25 fp32 columns are 3.2e9 bytes; from 2^26 on they pass 32 bits."""
+    lib = _native.attn_lib()
+    for out, W in ((200, 256), (128, 128)):
+        _refuses(lib.agpt_act8_wgrad(P, ld, 0, P, P, 0, P, P, P, 1 << 40, 300, out, W, None), UNS, "2^25")
+    _refuses(lib.agpt_act8_relu_wgrad(P, ld, 0, P, P + (1 << 40), P, P, 0, P, P, P, 1 << 40, 1, 128, 64, None), UNS, "2^25")
+
+
 @pytest.mark.parametrize("kw,part", [(dict(out=66), "multiple of 32"), (dict(ld=66), "16-byte"), (dict(dy=P + 8), "16-byte"),
                                      (dict(hc=None), "null"), (dict(dh=None), "null"), (dict(dh=P), "overlap"),
                                      (dict(hc=P + 8), "16-byte")])
