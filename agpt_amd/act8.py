@@ -26,6 +26,12 @@ class Act8:
     W: int
     relu: bool
 
+    def __post_init__(self):
+        n, device = -(-self.T // 8) * 8 * self.W, self.codes.device
+        for name, t, want in (("codes", self.codes, n), ("scales", self.scales, n // BLOCK)):
+            if t.dtype != torch.uint8 or t.numel() != want or not t.is_contiguous() or t.device != device:
+                raise ValueError(f"{name} must be {want} contiguous bytes on the codes' device")
+
     @property
     def device(self):
         return self.codes.device

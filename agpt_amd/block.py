@@ -72,8 +72,14 @@ def _check_apart(name: str, out, *inputs) -> None:
             raise ValueError(f"{name} must not overlap an input")
 
 
+_MAX_WIDTH = 2**31 - 1
+
+
 def _rows(name: str, t) -> int:
-    """The row stride, in elements, of a 2-D tensor whose rows are contiguous."""
+    """The row stride, in elements, of a 2-D tensor whose rows are contiguous
+    (and whose width is an int of the C entry points)."""
+    if t.dim() == 2 and t.shape[1] > _MAX_WIDTH:
+        raise ValueError(f"{name} is wider than 2^31 - 1")
     if t.dim() == 2 and t.numel() == 0:
         return max(1, t.shape[1])
     if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):

@@ -589,6 +589,7 @@ __global__ __launch_bounds__(kList) void direct_kernel(const T* __restrict__ dx,
   }
 }
 
+constexpr int kMaxWidth = 1 << 30;  // columns and steps past the last one stay in 32 bits
 constexpr int64_t kMaxCount = 0x7fffffff - 4096;  // places and steps past the last one stay in 32 bits
 
 int digit_bits(int64_t V, int* passes) {
@@ -653,6 +654,7 @@ extern "C" int agpt_embed_fwd(const void* table, const void* tokens, int token_b
                               int64_t V, int D, int dtype, void* stream) {
   const char* what = "agpt_embed_fwd";
   if (T < 0 || V < 1 || D < 1) return invalid(what, "T < 0, V < 1 or D < 1");
+  if (D > kMaxWidth) return invalid(what, "D must be at most 2^30");
   if (token_bits != 32 && token_bits != 64) return invalid(what, "token_bits must be 32 or 64");
   if (dtype != AGPT_DTYPE_F32 && dtype != AGPT_DTYPE_BF16) return invalid(what, "unknown dtype");
   if (T == 0) return AGPT_OK;
@@ -763,6 +765,7 @@ extern "C" int agpt_embed_bwd(const void* dx, int64_t ld_dx, const int32_t* plan
   const char* what = "agpt_embed_bwd";
   if (const int rc = check_counts(what, T, V)) return rc;
   if (D < 1 || ld_dx < D) return invalid(what, "D < 1 or a row stride smaller than D");
+  if (D > kMaxWidth) return invalid(what, "D must be at most 2^30");
   if (dtype != AGPT_DTYPE_F32 && dtype != AGPT_DTYPE_BF16) return invalid(what, "unknown dtype");
   if (!d_table || (T > 0 && (!dx || !plan || !workspace))) return invalid(what, "null pointer");
   const int es = dtype == AGPT_DTYPE_F32 ? 4 : 2;
@@ -831,6 +834,7 @@ extern "C" int agpt_embed_bwd_tokens(const void* dx, int64_t ld_dx, const void* 
   const char* what = "agpt_embed_bwd_tokens";
   if (const int rc = check_counts(what, T, V)) return rc;
   if (D < 1 || ld_dx < D) return invalid(what, "D < 1 or a row stride smaller than D");
+  if (D > kMaxWidth) return invalid(what, "D must be at most 2^30");
   if (token_bits != 32 && token_bits != 64) return invalid(what, "token_bits must be 32 or 64");
   if (dtype != AGPT_DTYPE_F32 && dtype != AGPT_DTYPE_BF16) return invalid(what, "unknown dtype");
   if (!d_table || !workspace || (T > 0 && (!dx || !tokens))) return invalid(what, "null pointer");

@@ -28,7 +28,8 @@ def embed_fwd(tokens, table, scale: float = 1.0, out=None):
     bits = _tokens(tokens)
     _check_cuda("table", table, tokens.device)
     dt = _dtype("table", table)
-    if table.dim() != 2 or not table.is_contiguous() or table.shape[0] < 1 or table.shape[1] < 1:
+    _rows("table", table)
+    if not table.is_contiguous() or table.shape[0] < 1 or table.shape[1] < 1:
         raise ValueError("table must be a contiguous [V, D] tensor, V and D at least 1")
     T, (V, D) = tokens.shape[0], table.shape
     if out is None:

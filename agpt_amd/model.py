@@ -193,7 +193,7 @@ class _Kept:
     def wgrad(self, tensors, dy, bias: bool):
         """(dw, db or None) of the layer from the saved tensors."""
         if self.shape is not None:
-            return act8.wgrad(dy, self.act(tensors), bias)
+            return act8.wgrad(dy.contiguous(), self.act(tensors), bias)
         db = None
         if bias:
             db = _col_sum(dy) if dy.shape[1] < 128 else dy.sum(0)

@@ -33,7 +33,7 @@ def _refuses(rc, code, part):
 
 @pytest.mark.parametrize("kw,part", [
     (dict(T=-1), "T < 0"), (dict(V=0), "V < 1"), (dict(D=0), "D < 1"), (dict(bits=16), "token_bits"),
-    (dict(dtype=7), "dtype"), (dict(table=None), "null"), (dict(tokens=None), "null"), (dict(x=None), "null"),
+    (dict(D=2**30 + 1), "2^30"), (dict(dtype=7), "dtype"), (dict(table=None), "null"), (dict(tokens=None), "null"), (dict(x=None), "null"),
     (dict(tokens=P + 4, bits=64), "aligned")])
 def test_embed_fwd_refuses(kw, part):
     a = dict(table=P, tokens=P, bits=32, x=P, T=3, V=5, D=8, dtype=0)
@@ -55,7 +55,7 @@ def test_embed_plan_refuses(kw, part):
 
 @pytest.mark.parametrize("kw,part", [
     (dict(T=-1), "T < 0"), (dict(V=0), "V < 1"), (dict(D=0), "D < 1"), (dict(ld=7), "row stride"),
-    (dict(dtype=2), "dtype"), (dict(dx=None), "null"), (dict(plan=None), "null"), (dict(dE=None), "null"),
+    (dict(D=2**30 + 8, ld=2**31), "2^30"), (dict(dtype=2), "dtype"), (dict(dx=None), "null"), (dict(plan=None), "null"), (dict(dE=None), "null"),
     (dict(ws=None), "null"), (dict(n=3), "workspace"), (dict(dx=P + 2), "aligned")])
 def test_embed_bwd_refuses(kw, part):
     a = dict(dx=P, ld=8, plan=P, dE=P, ws=P, n=1 << 20, T=300, V=5, D=8, dtype=0)
@@ -66,7 +66,7 @@ def test_embed_bwd_refuses(kw, part):
 
 @pytest.mark.parametrize("kw,part", [
     (dict(T=-1), "T < 0"), (dict(V=0), "V < 1"), (dict(V=2**31 - 1), "2^31"), (dict(D=0), "D < 1"),
-    (dict(ld=7), "row stride"), (dict(bits=8), "token_bits"), (dict(dtype=2), "dtype"), (dict(dx=None), "null"),
+    (dict(D=2**30 + 8, ld=2**31), "2^30"), (dict(ld=7), "row stride"), (dict(bits=8), "token_bits"), (dict(dtype=2), "dtype"), (dict(dx=None), "null"),
     (dict(tokens=None), "null"), (dict(dE=None), "null"), (dict(ws=None), "null"), (dict(n=3), "workspace"),
     (dict(dx=P + 2), "aligned"), (dict(tokens=P + 2), "aligned")])
 def test_embed_bwd_tokens_refuses(kw, part):
@@ -170,6 +170,23 @@ def test_sizes():
     T = 2**31 - 5000  # sizes past 32 bits
     assert lib.agpt_embed_plan_workspace_bytes(T, 65) > 8 * T
     assert lib.agpt_act8_code_bytes(1 << 32, 512) == 1 << 41
+
+
+def test_checkpoint_of_other_sizes_is_refused():
+    """Act8 is public: bytes that do not fit its sizes never reach a kernel."""
+    codes, scales = torch.zeros(16 * 64, dtype=torch.uint8), torch.zeros(32, dtype=torch.uint8)
+    assert act8.Act8(codes, scales, 9, 64, False).device.type == "cpu"
+    for args in ((codes[:-1], scales, 9, 64), (codes, scales[:-1], 9, 64), (codes, scales, 17, 64), (codes, scales, 9, 96),
+                 (codes.int(), scales, 9, 64), (torch.zeros(2048, dtype=torch.uint8)[::2], scales, 9, 64),
+                 (codes, scales.to("meta"), 9, 64)):
+        with pytest.raises(ValueError):
+            act8.Act8(*args, False)
+
+
+def test_widths_past_an_int_are_refused():
+    """Before they are cut to the C entry points' 32 bits."""
+    with pytest.raises(ValueError, match="wider"):
+        block._rows("x", torch.empty(1, 2**32 + 64, device="meta"))
 
 
 def test_python_mirror_needs_a_gpu():
