@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .block import _check_apart, _check_cuda, _dtype, _launch, _ptr, _rows
+from .block import _MAX_WIDTH, _check_apart, _check_cuda, _dtype, _launch, _ptr, _rows
 
 _BITS = {torch.int32: 32, torch.int64: 64}
 
@@ -28,10 +28,11 @@ def embed_fwd(tokens, table, scale: float = 1.0, out=None):
     bits = _tokens(tokens)
     _check_cuda("table", table, tokens.device)
     dt = _dtype("table", table)
-    _rows("table", table)
-    if not table.is_contiguous() or table.shape[0] < 1 or table.shape[1] < 1:
-        raise ValueError("table must be a contiguous [V, D] tensor, V and D at least 1")
+    if table.dim() != 2 or not table.is_contiguous():
+        raise ValueError("table must be a contiguous [V, D] tensor")
     T, (V, D) = tokens.shape[0], table.shape
+    if V < 1 or not 1 <= D <= _MAX_WIDTH:
+        raise ValueError("the table's V and D must be at least 1, D below 2^31")
     if out is None:
         out = torch.empty(T, D, device=table.device, dtype=table.dtype)
     else:
